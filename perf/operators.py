@@ -373,7 +373,7 @@ def _fork(s):
     free = torch.nonzero(ref == 0).flatten().to(torch.int32)
     rank = (torch.cumsum(fresh.flatten(), 0) - 1).view(slots, width)
     got = fresh & (rank < free.numel())
-    table = torch.where(got, free[torch.where(got, rank, 0)], table)
+    table[got] = free[rank[got]]
     ref = ref + _counts(torch.where(got, table, -1), c["n_blocks"])
     copy = got & tail
     s["caches"][:, table[copy].long()] = s["caches"][:, old[copy].long()]
