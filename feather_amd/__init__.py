@@ -17,7 +17,9 @@ from .packers.fp8 import pack_fp8_tensor, unpack_fp8_tensor  # noqa: F401
 from .packers.fp16 import pack_fp16_tensor, unpack_fp16_tensor  # noqa: F401
 from .routines.attention import (flash_attention_fp8_acc_fp32_gpu, flash_attention_fp8_e4m3_acc_fp32_gpu,  # noqa: F401
                                  flash_attention_fp8_e5m2_acc_fp32_gpu)
-from .routines.paged_attention import paged_attention_fp8_acc_fp32_gpu  # noqa: F401
+from .routines.paged_attention import (paged_attention_fp8_acc_fp32_gpu,  # noqa: F401
+                                       paged_chunk_attention_fp8_acc_fp32_gpu)
+from .routines.paged_cache import paged_cache_compact, paged_cache_fork  # noqa: F401
 from .routines import dot as _dot, gemv as _gemv
 
 __version__ = "0.1.0"

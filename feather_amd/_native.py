@@ -16,12 +16,14 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libfeather_hip.so")
 
 OK, EINVAL, EMODE, ESHAPE, ELAUNCH = 0, -1, -2, -3, -4
-ABI_VERSION = 10400   # FEATHER_HIP_VERSION of the include/feather_hip.h these signatures were written against
+ABI_VERSION = 10500   # FEATHER_HIP_VERSION of the include/feather_hip.h these signatures were written against
 E5M2, E4M3 = 0, 1
 ROUND_RNE, ROUND_TRUNC = 0, 1
 SEM_KERNEL, SEM_IEEE = 0, 1
 OUT_F32, OUT_F16 = 0, 1
 TAIL_MASK, TAIL_REFERENCE = 0, 1
+CHUNK_OUT_F32, CHUNK_OUT_F16, CHUNK_OUT_PACKED = 0, 1, 2
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
 
 _MODES = {"E5M2": E5M2, "E4M3": E4M3}
 
@@ -59,6 +61,14 @@ SIGNATURES = {
     "feather_add_rmsnorm_pack": (_i32, [_vp, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _f32, _i32, _vp]),
     "feather_rope_append": (_i32, [_vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
                                    _i64, _i64, _f32, _i32, _vp]),
+    "feather_paged_chunk_attn_scratch_bytes": (_i64, [_i64] * 7),
+    "feather_paged_chunk_attn_fp8": (_i32, [_vp] * 7 + [_i32, _i32, _vp] + [_i64] * 10 + [_i32, _i32, _f32, _vp]),
+    "feather_rope_append_chunk": (_i32, [_vp, _i32, _i64, _vp, _vp, _vp, _vp, _f32, _i64, _i32] + [_vp] * 6 + [_i32]
+                                  + [_i64] * 8 + [_i32, _vp]),
+    "feather_paged_cache_fork_scratch_bytes": (_i64, [_i64, _i64]),
+    "feather_paged_cache_fork": (_i32, [_vp, _i64, _i64] + [_vp] * 10 + [_i64] * 4 + [_vp]),
+    "feather_paged_cache_compact_scratch_bytes": (_i64, [_i64]),
+    "feather_paged_cache_compact": (_i32, [_vp, _i64, _i64] + [_vp] * 7 + [_i64, _i64, _vp]),
 }
 
 

@@ -1,7 +1,7 @@
-"""Single-query attention over a paged FP8 KV cache (decode step).  The reference
+"""Attention over a paged FP8 KV cache: one query per sequence (decode step, ``csrc/paged_attention.hip``) or a
+chunk of new rows per sequence (``csrc/paged_chunk_attention.hip``), and the writer of the cache.  The reference
 has no paged attention; numerics follow its flash-attention kernel (decode by
-mode, fp32 scores and softmax, P rounded to fp16, fp32 output) and the kernel is
-``csrc/paged_attention.hip``.
+mode, fp32 scores and softmax, P rounded to fp16, fp32 output).
 """
 from __future__ import annotations
 
@@ -11,7 +11,9 @@ import torch
 
 from .. import _native as N
 
-__all__ = ["paged_attention_fp8_acc_fp32_gpu", "paged_cache_write"]
+__all__ = ["paged_attention_fp8_acc_fp32_gpu", "paged_chunk_attention_fp8_acc_fp32_gpu", "paged_cache_write"]
+
+_CHUNK_OUT = {torch.float32: N.CHUNK_OUT_F32, torch.float16: N.CHUNK_OUT_F16, torch.uint32: N.CHUNK_OUT_PACKED}
 
 
 def paged_attention_fp8_acc_fp32_gpu(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -71,6 +73,82 @@ def paged_attention_fp8_acc_fp32_gpu(q: torch.Tensor, k_cache: torch.Tensor, v_c
            N.ptr(context_lens), N.ptr(out), N.ptr(packed) if packed is not None else None, N.ptr(scratch), n_seq,
            n_q_heads, n_kv_heads, d, block_size, max_blocks, n_blocks, max_ctx, code, float(scale))
     return (out, packed.view(torch.uint32)) if return_packed else out
+
+
+def paged_chunk_attention_fp8_acc_fp32_gpu(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                                           block_tables: torch.Tensor, cu_seqlens: torch.Tensor,
+                                           ctx_lens: torch.Tensor, *, mode: str = "E5M2", scale: float | None = None,
+                                           causal: bool = True, max_q_len: int | None = None,
+                                           out_dtype: torch.dtype = torch.float32,
+                                           out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of the new rows of a ragged batch over the paged cache that already holds their K and V.
+
+    q             ``[total_rows, n_q_heads, d/4]`` packed words (as :func:`rope_append_chunk` returns them)
+    k_cache       ``[n_blocks, n_kv_heads, block_size, d/4]`` packed words (``v_cache`` alike)
+    block_tables  ``[n_seq, max_blocks]`` int32
+    cu_seqlens    ``[n_seq + 1]`` int32: sequence ``s`` has rows ``cu[s] .. cu[s+1]-1``
+    ctx_lens      ``[n_seq]`` int32: tokens in the cache, the sequence's new rows among them (its last ones)
+    causal        row ``i`` of ``n`` sees positions ``0 .. ctx - n + i``; without it every row sees all ``ctx``
+                  positions (cross attention to cached states of any length)
+    max_q_len     a bound of the rows of a sequence, if known; it only helps to choose the kernels
+    out_dtype     float32 or float16 ``[total_rows, n_q_heads, d]``, or uint32: packed FP8 words
+                  ``[total_rows, n_q_heads * d / 4]`` of ``mode``, the operand of a following packed GEMV
+    out           optional result tensor of that type and shape; rows outside every sequence keep what it held
+                  (without ``out`` they are zero)
+    ``d`` is 64, 128, 256 or 512; any number of query heads per KV head.  A row that sees no position gets zeros.
+    Table entries that are not blocks of the cache are read as the last block."""
+    code = N.mode_code(mode)
+    q, k_cache, v_cache = N.as_words(q, "q"), N.as_words(k_cache, "k_cache"), N.as_words(v_cache, "v_cache")
+    if q.dim() != 3 or k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError("expected q [total_rows, n_q_heads, d/4] and k_cache/v_cache [n_blocks, n_kv_heads, block_size, d/4]")
+    total, n_q_heads, dw = q.shape
+    n_blocks, n_kv_heads, block_size, dw2 = k_cache.shape
+    if dw != dw2:
+        raise ValueError(f"head dim mismatch: q has {dw} words per head, cache has {dw2}")
+    d = 4 * dw
+    if d not in (64, 128, 256, 512):
+        raise ValueError(f"head dim {d} not supported: 64, 128, 256 or 512")
+    if n_kv_heads < 1 or n_q_heads < 1 or n_q_heads % n_kv_heads != 0:
+        raise ValueError(f"n_q_heads={n_q_heads} must be a multiple of n_kv_heads={n_kv_heads}")
+    if n_blocks < 1 or block_size < 1:
+        raise ValueError("the cache must hold at least one block")
+    for name, t, dims in (("block_tables", block_tables, 2), ("cu_seqlens", cu_seqlens, 1), ("ctx_lens", ctx_lens, 1)):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != dims:
+            raise ValueError(f"{name} must be a {dims}-D int32 tensor")
+        if t.device != q.device:
+            raise ValueError(f"{name} is on {t.device}, q on {q.device}")
+    n_seq = ctx_lens.shape[0]
+    if block_tables.shape[0] != n_seq or cu_seqlens.shape[0] != n_seq + 1:
+        raise ValueError("block_tables must be [n_seq, max_blocks], cu_seqlens [n_seq + 1] and ctx_lens [n_seq]")
+    if k_cache.device != q.device or v_cache.device != q.device:
+        raise ValueError("q and the caches must be on the same device")
+    if scale is None:
+        scale = 1.0 / math.sqrt(d)
+    if not 0 < scale < math.inf:
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    max_q_len = 0 if max_q_len is None else int(max_q_len)
+    if max_q_len < 0:
+        raise ValueError(f"max_q_len must not be negative, got {max_q_len}")
+    kind = _CHUNK_OUT.get(out_dtype)
+    if kind is None:
+        raise ValueError(f"out_dtype must be float32, float16 or uint32 (packed words), got {out_dtype}")
+    shape = (total, n_q_heads * dw) if kind == N.CHUNK_OUT_PACKED else (total, n_q_heads, d)
+    fill = 1 if out is None else 0
+    if out is None:
+        out = torch.empty(shape, dtype=out_dtype, device=q.device)
+    elif (not isinstance(out, torch.Tensor) or out.dtype != out_dtype or tuple(out.shape) != shape
+          or out.device != q.device or not out.is_contiguous()):
+        raise ValueError(f"out must be a contiguous {out_dtype} tensor of shape {shape} on {q.device}")
+    block_tables, cu_seqlens, ctx_lens = block_tables.contiguous(), cu_seqlens.contiguous(), ctx_lens.contiguous()
+    max_blocks = block_tables.shape[1]
+    nbytes = N.lib().feather_paged_chunk_attn_scratch_bytes(n_seq, total, n_q_heads, n_kv_heads, d, max_blocks * block_size,
+                                                            max_q_len)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes > 0 else None
+    N.call(q.device, "feather_paged_chunk_attn_fp8", N.ptr(q), N.ptr(k_cache), N.ptr(v_cache), N.ptr(block_tables),
+           N.ptr(cu_seqlens), N.ptr(ctx_lens), N.ptr(out), kind, fill, N.ptr(scratch) if scratch is not None else None,
+           max(nbytes, 0), n_seq, total, n_q_heads, n_kv_heads, d, block_size, max_blocks, n_blocks, max_q_len,
+           1 if causal else 0, code, float(scale))
+    return out
 
 
 def paged_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,

@@ -3,15 +3,18 @@ packed routines.  The reference quantises on the CPU (``pack_fp8_tensor``,
 feather/packers/fp8.py:260-281) and has no device-side producer; here the rounding chain
 fp32 -> fp16 -> FP8 (round to nearest even twice, i.e. ``pack_fp8_tensor(x.half())``) and the
 packing run inside the kernel that computes the values (``csrc/pack.hip``,
-``csrc/decode_step.hip``, the SwiGLU epilogue of ``csrc/gemv_batched.hip``).
+``csrc/decode_step.hip``, ``csrc/rope_chunk.hip``, the SwiGLU epilogue of ``csrc/gemv_batched.hip``).
 """
 from __future__ import annotations
+
+import math
 
 import torch
 
 from .. import _native as N
 
-__all__ = ["quant_pack_f32", "add_rmsnorm_pack", "rope_append", "gemv_fp8_batched_swiglu"]
+__all__ = ["quant_pack_f32", "add_rmsnorm_pack", "rope_append", "rope_append_chunk", "rotary_frequencies",
+           "gemv_fp8_batched_swiglu"]
 
 
 def _f32(t: torch.Tensor, name: str, shape=None) -> torch.Tensor:
@@ -108,6 +111,112 @@ def rope_append(qkv: torch.Tensor, ctx_lens: torch.Tensor, block_tables: torch.T
            n_blocks, float(rope_theta), code)
     res = (qp.view(torch.uint32), ctx_after, status)
     return res + (rot,) if return_f32 else res
+
+
+def rotary_frequencies(rot_dim: int, *, theta: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                       original_context: int | None = None, low: float = 1.0, high: float = 32.0,
+                       device=None) -> torch.Tensor:
+    """Turns per position of the ``rot_dim / 2`` rotated pairs, float64: ``f_j = theta^(-2j / rot_dim) / (2 pi)``.
+
+    scaling   ``"none"``; ``"linear"``: every ``f_j / factor`` (positions interpolated); ``"base"``: theta is raised to
+              ``theta * factor^(rot_dim / (rot_dim - 2))``, which stretches the slowest pair by ``factor`` and leaves the
+              fastest; ``"by_parts"``: pairs that make fewer than ``low`` turns over ``original_context`` positions are
+              divided by ``factor``, those above ``high`` turns are kept, with a linear ramp between
+    device    where the table goes (default: the current HIP device)"""
+    rot_dim = int(rot_dim)
+    if rot_dim < 2 or rot_dim % 2 != 0:
+        raise ValueError(f"rot_dim must be a positive even number, got {rot_dim}")
+    if not (0 < theta < math.inf and 0 < factor < math.inf):
+        raise ValueError("theta and factor must be positive")
+    if scaling not in ("none", "linear", "base", "by_parts"):
+        raise ValueError(f"scaling must be 'none', 'linear', 'base' or 'by_parts', got {scaling!r}")
+    if scaling == "base":
+        if rot_dim < 4:
+            raise ValueError("scaling='base' needs rot_dim >= 4")
+        theta = theta * factor ** (rot_dim / (rot_dim - 2))
+    j = torch.arange(rot_dim // 2, dtype=torch.float64)
+    f = theta ** (-2.0 * j / rot_dim) / (2.0 * math.pi)
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "by_parts":
+        if original_context is None or original_context < 1 or not 0 <= low < high:
+            raise ValueError("scaling='by_parts' needs original_context >= 1 and 0 <= low < high")
+        keep = ((original_context * f - low) / (high - low)).clamp(0.0, 1.0)
+        f = f * (keep + (1.0 - keep) / factor)
+    return f.to(N.require_gpu() if device is None else device)
+
+
+_ROPE_LAYOUTS = {"half": N.ROPE_HALF, "interleaved": N.ROPE_INTERLEAVED}
+
+
+def rope_append_chunk(qkv: torch.Tensor, cu_seqlens: torch.Tensor, start_pos: torch.Tensor, block_tables: torch.Tensor,
+                      k_cache: torch.Tensor, v_cache: torch.Tensor, *, n_q_heads: int, freq: torch.Tensor,
+                      amplitude: float = 1.0, layout: str = "half", mode: str = "E4M3", return_f32: bool = False):
+    """Rotary positions for the new rows of a ragged batch, q packed to FP8, k and v encoded into the paged cache.
+
+    qkv           ``[total_rows, (n_q + 2 n_kv) * d]`` float32 or float16: q heads, k heads, v heads (rows may be strided)
+    cu_seqlens    ``[n_seq + 1]`` int32; row ``cu[s] + i`` is at position ``start_pos[s] + i``
+    block_tables  ``[n_seq, max_blocks]`` int32
+    freq          ``[rot_dim / 2]`` float64 turns per position (:func:`rotary_frequencies`); dims from ``rot_dim`` on pass
+                  as they are.  ``rot_dim`` is a multiple of 8, at most ``d``
+    amplitude     factor of the rotated dims of q and k (attention temperature of scaled contexts)
+    layout        ``"half"``: element ``j`` turns with ``j + rot_dim / 2``; ``"interleaved"``: ``2j`` with ``2j + 1``
+    Returns ``(q_packed [total_rows, n_q, d/4], ctx_after [n_seq], status [n_seq])`` and with ``return_f32`` also the
+    fp32 values ``[total_rows, n_q + 2 n_kv, d]`` the codes were rounded from.  ``ctx_after`` counts the cached tokens up
+    to the first that could not be written; ``status``: 0 all written, 1 a position has no table entry, 2 a table entry
+    is not a block of the cache.  Rows outside every sequence give zeros and are not appended."""
+    code = N.mode_code(mode)
+    if layout not in _ROPE_LAYOUTS:
+        raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}")
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        N.as_words(t, name)
+        if not t.is_contiguous():
+            raise ValueError(f"{name} is written in place and must be contiguous")
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError("expected k_cache/v_cache [n_blocks, n_kv_heads, block_size, d/4]")
+    n_blocks, n_kv, block_size, dw = k_cache.shape
+    d, n_q = 4 * dw, int(n_q_heads)
+    if n_q < 0 or n_blocks < 1 or n_kv < 1 or block_size < 1:
+        raise ValueError("the cache must hold at least one block, and n_q_heads must not be negative")
+    heads = n_q + 2 * n_kv
+    if not isinstance(qkv, torch.Tensor) or qkv.dtype not in (torch.float32, torch.float16) or not qkv.is_cuda:
+        raise ValueError("qkv must be a float32 or float16 tensor on the device")
+    if qkv.dim() != 2 or qkv.shape[1] != heads * d:
+        raise ValueError(f"qkv must be [total_rows, {heads * d}], got {tuple(qkv.shape)}")
+    total = qkv.shape[0]
+    if total > 1 and (qkv.stride(1) != 1 or qkv.stride(0) % 4 != 0 or qkv.stride(0) < heads * d) or qkv.data_ptr() % 16 != 0:
+        qkv = qkv.contiguous() if qkv.data_ptr() % 16 == 0 else qkv.clone(memory_format=torch.contiguous_format)
+    row_stride = qkv.stride(0) if total > 1 else heads * d
+    if qkv.stride(1) != 1:
+        qkv, row_stride = qkv.contiguous(), heads * d
+    _i32(cu_seqlens, "cu_seqlens")
+    n_seq = cu_seqlens.numel() - 1
+    if cu_seqlens.dim() != 1 or n_seq < 0:
+        raise ValueError("cu_seqlens must be [n_seq + 1]")
+    _i32(start_pos, "start_pos", (n_seq,))
+    _i32(block_tables, "block_tables")
+    if block_tables.dim() != 2 or block_tables.shape[0] != n_seq:
+        raise ValueError("block_tables must be [n_seq, max_blocks]")
+    if not isinstance(freq, torch.Tensor) or freq.dtype != torch.float64 or freq.dim() != 1 or not freq.is_contiguous():
+        raise ValueError("freq must be a contiguous 1-D float64 tensor (rotary_frequencies)")
+    rot = 2 * freq.numel()
+    if rot % 8 != 0 or rot > d:
+        raise ValueError(f"rot_dim={rot} (two per frequency) must be a multiple of 8 and at most the head dim {d}")
+    if not math.isfinite(amplitude):
+        raise ValueError(f"amplitude must be finite, got {amplitude}")
+    _same_device(qkv, cu_seqlens, start_pos, block_tables, k_cache, v_cache, freq)
+    dev = qkv.device
+    qp = torch.empty((total, n_q, dw), dtype=torch.uint32, device=dev)
+    ctx_after = torch.empty((n_seq,), dtype=torch.int32, device=dev)
+    status = torch.empty((n_seq,), dtype=torch.int32, device=dev)
+    rotated = torch.empty((total, heads, d), dtype=torch.float32, device=dev) if return_f32 else None
+    N.call(dev, "feather_rope_append_chunk", N.ptr(qkv), 1 if qkv.dtype == torch.float16 else 0, row_stride,
+           N.ptr(cu_seqlens), N.ptr(start_pos), N.ptr(block_tables), N.ptr(freq), float(amplitude), rot,
+           _ROPE_LAYOUTS[layout], N.ptr(qp), N.ptr(k_cache), N.ptr(v_cache), N.ptr(ctx_after), N.ptr(status),
+           N.ptr(rotated) if rotated is not None else None, 1, n_seq, total, n_q, n_kv, d, block_size,
+           block_tables.shape[1], n_blocks, code)
+    res = (qp, ctx_after, status)
+    return res + (rotated,) if return_f32 else res
 
 
 def gemv_fp8_batched_swiglu(w_gate_up: torch.Tensor, x: torch.Tensor, inter: int, K: int, nvec: int, *,

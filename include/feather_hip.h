@@ -52,10 +52,17 @@ extern "C" {
 #define FEATHER_TAIL_REFERENCE 1  /* keys past seq_len in the last 64-key tile count as zero rows
                                      (attention.py:57-59) */
 
+#define FEATHER_CHUNK_OUT_F32 0    /* output of feather_paged_chunk_attn_fp8 */
+#define FEATHER_CHUNK_OUT_F16 1
+#define FEATHER_CHUNK_OUT_PACKED 2
+
+#define FEATHER_ROPE_HALF 0        /* element j turns with j + rot_dim / 2 */
+#define FEATHER_ROPE_INTERLEAVED 1 /* element 2j turns with 2j + 1 */
+
 /* Library version (major * 10000 + minor * 100 + patch); FEATHER_HIP_VERSION is the version of this header.
  * A change of any signature or struct below raises the minor number: a binding must refuse a library whose
  * feather_version() differs from the header it was written against in major or minor. */
-#define FEATHER_HIP_VERSION 10400
+#define FEATHER_HIP_VERSION 10500
 int feather_version(void);
 
 /* Message for the last non-zero return code on this thread ("" if none). */
@@ -312,6 +319,90 @@ int feather_rope_append(const void *qkv_f32, int64_t n_part, int64_t part_stride
                         void *seq_status, void *rot_f32, int64_t batch, int64_t n_q_heads, int64_t n_kv_heads, int64_t d,
                         int64_t block_size, int64_t max_blocks, int64_t n_blocks, float rope_theta, int mode,
                         void *stream);
+
+/* ---- new tokens in chunks over the paged cache (no reference counterpart) ----
+ *
+ * A batch of n_seq sequences brings cu_seqlens[s+1] - cu_seqlens[s] new rows each (cu_seqlens [n_seq + 1] int32 on
+ * the device, non-decreasing, offsets into total_rows rows; values outside [0, total_rows] are clamped): drafted tokens
+ * to verify, chunks of prompts, single tokens, in any mix.  Rows outside every sequence (before cu[0], from cu[n_seq]
+ * on) are set to zero with fill = 1 and left as they were with fill = 0.
+ *
+ * feather_paged_chunk_attn_fp8: attention of the new rows over the cache that already holds them.
+ *   q            [total_rows, n_q_heads, d/4] packed words
+ *   k_cache      [n_blocks, n_kv_heads, block_size, d/4] words (v_cache same)
+ *   block_tables [n_seq, max_blocks] int32
+ *   ctx_lens     [n_seq] int32: tokens in the cache, the sequence's new rows among them (they are its last ones)
+ *   out          out_kind FEATHER_CHUNK_OUT_F32 / _F16: [total_rows, n_q_heads, d]; _PACKED: [total_rows, n_q_heads * d/4]
+ *                words of `mode` (fp32 -> fp16 -> FP8, as feather_quant_pack_f32)
+ *   causal       1: row i of n sees positions 0 .. ctx_lens[s] - n + i (a row that sees none gets a zero result);
+ *                0: every row sees all ctx_lens[s] positions (cross attention to cached states of any length)
+ *   max_q_len    a bound of the rows of a sequence if the caller knows one, or 0.  It only chooses the kernels: a wrong
+ *                value costs time, never rows.
+ *   scratch      feather_paged_chunk_attn_scratch_bytes(n_seq, total_rows, n_q_heads, n_kv_heads, d, max_blocks * block_size,
+ *                max_q_len) bytes, 16-byte aligned: the key loops of few rows are cut into ranges that run side by side.
+ *                NULL or a smaller buffer: fewer ranges, the same result up to the order of fp32 additions.  Nothing is
+ *                kept in it between calls; calls that overlap need one each.
+ * d in {64, 128, 256, 512}, any n_q_heads / n_kv_heads ratio.  Query head h reads KV head h / (n_q_heads / n_kv_heads).
+ * Lengths are clamped to [0, max_blocks * block_size]; a table entry outside [0, n_blocks) within the context is read as
+ * the last block; entries and cache slots past the context are not used, whatever they hold.  A position that a row
+ * does not see has no influence on it, also where its K or V is infinite or NaN.  scale > 0. */
+int64_t feather_paged_chunk_attn_scratch_bytes(int64_t n_seq, int64_t total_rows, int64_t n_q_heads, int64_t n_kv_heads,
+                                               int64_t d, int64_t max_ctx, int64_t max_q_len);
+int feather_paged_chunk_attn_fp8(const void *q, const void *k_cache, const void *v_cache, const void *block_tables,
+                                 const void *cu_seqlens, const void *ctx_lens, void *out, int out_kind, int fill,
+                                 void *scratch, int64_t scratch_bytes, int64_t n_seq, int64_t total_rows, int64_t n_q_heads,
+                                 int64_t n_kv_heads, int64_t d, int64_t block_size, int64_t max_blocks, int64_t n_blocks,
+                                 int64_t max_q_len, int causal, int mode, float scale, void *stream);
+
+/* feather_rope_append_chunk: the rows' projections become the operands of feather_paged_chunk_attn_fp8.
+ *   qkv          [total_rows, (n_q + 2 n_kv) * d] fp32 (src_f16 = 0) or fp16 (1): q heads, k heads, v heads; rows are
+ *                row_stride elements apart (a multiple of 4)
+ *   start_pos    [n_seq] int32 position of each sequence's first row; row i is at start_pos[s] + i
+ *   freq_f64     [rot_dim / 2] turns per position (theta^(-2j / rot_dim) / (2 pi) for the plain table); the first rot_dim
+ *                dims of every q and k head are rotated by 2 pi * position * freq (computed in 64 bits) and multiplied by
+ *                `amplitude`, the others pass as they are.  rot_dim % 8 == 0, 0 <= rot_dim <= min(d, 512); d % 8 == 0.
+ *   layout       FEATHER_ROPE_HALF or FEATHER_ROPE_INTERLEAVED
+ *   q_packed     [total_rows, n_q, d/4] words; k and v are encoded into the cache at their positions.  A position outside
+ *                [0, max_blocks * block_size), or whose table entry is not a block, is not written.  Two rows must not
+ *                name the same slot.
+ *   ctx_after    [n_seq] tokens in the cache up to the first one that could not be written (start_pos + rows if all were)
+ *   seq_status   [n_seq] or NULL: 0 = all written, 1 = some position has no table entry, 2 = some entry is not a block
+ *   rot_f32      [total_rows, n_q + 2 n_kv, d] or NULL: the fp32 values the codes were rounded from */
+int feather_rope_append_chunk(const void *qkv, int src_f16, int64_t row_stride, const void *cu_seqlens, const void *start_pos,
+                              const void *block_tables, const void *freq_f64, float amplitude, int64_t rot_dim, int layout,
+                              void *q_packed, void *k_cache, void *v_cache, void *ctx_after, void *seq_status, void *rot_f32,
+                              int fill, int64_t n_seq, int64_t total_rows, int64_t n_q_heads, int64_t n_kv_heads, int64_t d,
+                              int64_t block_size, int64_t max_blocks, int64_t n_blocks, int mode, void *stream);
+
+/* ---- the pages of a cache as a pool (no reference counterpart) ----
+ *
+ * ref_counts [n_blocks] int32: how many table entries (and pins of the caller) hold a block; 0 = free.  caches_host is a
+ * HOST array of n_caches device pointers, every cache [n_blocks] blocks of block_bytes bytes (a multiple of 16): K and V
+ * of all layers that share the tables.  Tables, counts and lengths are read from their inputs and written to separate
+ * outputs; of the caches only blocks that were free are written.  n_blocks <= 4194304.
+ *
+ * feather_paged_cache_fork: slot i becomes a copy of slot parents[i] of the old state ([n_seq] int32; a value outside
+ * [0, n_seq) ends the slot: an empty row, length 0).  Blocks that a context fills are shared by all children.  The first child (lowest i) of a
+ * parent takes the rest of its row too; every other child gets a copy of the block its context ends in.  Then, if room
+ * ([n_seq] int32) is given, entries past the context are filled with fresh blocks until the row covers room[i] positions.
+ * Fresh blocks are the free ones (after the old rows have let go), lowest id first, in (slot, entry) order.  Entries that
+ * are not blocks come out as -1.  seq_status (or NULL): 0; 1 = room[i] beyond the table (filled to its end); 2 = an entry
+ * within the context is not a block; 3 = the pool ran out (missing entries are -1; a slot that lost the copy of its last
+ * block keeps its whole blocks as its length).  ref_counts must count the rows of block_tables.  n_seq <= 8192. */
+int64_t feather_paged_cache_fork_scratch_bytes(int64_t n_seq, int64_t n_blocks);
+int feather_paged_cache_fork(const void *const *caches_host, int64_t n_caches, int64_t block_bytes, const void *block_tables,
+                             const void *ctx_lens, const void *ref_counts, const void *parents, const void *room,
+                             void *tables_out, void *ctx_out, void *ref_out, void *seq_status, void *scratch, int64_t n_seq,
+                             int64_t max_blocks, int64_t block_size, int64_t n_blocks, void *stream);
+
+/* feather_paged_cache_compact: the n_live blocks with ref_counts > 0 move to ids 0 .. n_live - 1; blocks already there
+ * stay, the highest of the others goes into the lowest hole and so on.  block_map [n_blocks] is the new id of every
+ * old block (-1: free), n_live one int32; tables_out are the n_entries entries of block_tables under that map (-1 for
+ * what is not a block in use).  Data left above n_live is stale. */
+int64_t feather_paged_cache_compact_scratch_bytes(int64_t n_blocks);
+int feather_paged_cache_compact(const void *const *caches_host, int64_t n_caches, int64_t block_bytes, const void *block_tables,
+                                const void *ref_counts, void *tables_out, void *ref_out, void *block_map, void *n_live,
+                                void *scratch, int64_t n_entries, int64_t n_blocks, void *stream);
 
 #ifdef __cplusplus
 }
