@@ -30,12 +30,17 @@ struct ChunkArgs {
     const uint32_t *q, *k_cache, *v_cache;
     const int32_t *block_tables, *cu_seqlens, *ctx_lens;
     void *out;
-    float *part;            // partial results of the key ranges (z > 1)
+    float *part;            // partial results of the LDS kernel's key ranges (z_wide > 1), then the (maximum, sum) pairs
     int n_seq, total_rows, n_q_heads, n_kv_heads, group, block_size, max_blocks;
     uint32_t max_blk;       // last block of the cache: an entry outside the cache is read as this one
-    uint32_t div_mul;       // pos / block_size = umulhi(2 pos, div_mul) >> div_shift for 0 <= pos < 2^31
-    int div_shift;
-    int causal, z, out_kind, fill;
+    uint32_t div_mul, group_mul, kv_mul;   // x / size = umulhi(2 x, mul) >> shift for 0 <= x < 2^31 (block_size, group, n_kv_heads)
+    int div_shift, group_shift, kv_shift;
+    int causal, out_kind, fill;
+    int z_wide, z_narrow;             // most key ranges of a tile in either kernel
+    float per_group;                  // KV heads over the workgroups of the narrow kernel that the chip holds at once
+    int narrow_rows;                  // beside the LDS kernel: rows a sequence of the narrow one can have (0: it runs alone)
+    float *part_narrow;               // its partial results, then the (maximum, sum) pairs, then the keys per range
+    int col_split;                    // sequences of more columns than this take the LDS kernel, the others the narrow one
     float scale_log2e;
 };
 
@@ -53,34 +58,50 @@ struct ChunkTile {
 // 64 sequences are looked at per step, one memory round trip each.
 __device__ __forceinline__ int chunk_clamp_row(int r, int total) { return min(max(r, 0), total); }
 
-__device__ __forceinline__ bool chunk_find_tile(const ChunkArgs &a, int slot, int qt, ChunkTile &t) {
+__device__ __forceinline__ int chunk_row_of(const ChunkArgs &a, int col) { return (int)(__umulhi(2u * (uint32_t)col, a.group_mul) >> a.group_shift); }
+
+template <bool SUM = false>
+__device__ __forceinline__ bool chunk_find_tile(const ChunkArgs &a, int slot, int qt, ChunkTile &t, int sum_qt = 1, float *sum = nullptr) {
     const int lane = lane_id();
-    int below = 0;
+    t.seq = -1;
+    float keys = 0.f;       // SUM: the lane's share of the keys of all tiles of sum_qt columns (an estimate will do)
     for (int s0 = 0; s0 < a.n_seq; s0 += kWave) {
-        const int s = s0 + lane;
-        const bool hit = s < a.n_seq &&
-                         (int64_t)chunk_clamp_row(a.cu_seqlens[min(s, a.n_seq - 1)], a.total_rows) * a.group / qt + s <= slot;
-        const uint64_t m = __builtin_amdgcn_ballot_w64(hit);
-        below += __builtin_popcountll(m);
-        if (m != ~0ull) break;
+        const int s = min(s0 + lane, a.n_seq - 1);
+        const int r0 = a.cu_seqlens[s], r1 = a.cu_seqlens[s + 1], ctx = a.ctx_lens[s];
+        const int row0 = chunk_clamp_row(r0, a.total_rows);
+        const uint64_t m = __builtin_amdgcn_ballot_w64(s0 + lane < a.n_seq && row0 * a.group / qt + s <= slot);
+        if (m != 0) {
+            const int at = __builtin_popcountll(m) - 1;
+            t.seq = s0 + at;
+            t.row0 = __builtin_amdgcn_readlane(row0, at);
+            t.rows = max(chunk_clamp_row(__builtin_amdgcn_readlane(r1, at), a.total_rows) - t.row0, 0);
+            t.ctx = min(max(__builtin_amdgcn_readlane(ctx, at), 0), a.max_blocks * a.block_size);
+        }
+        if constexpr (SUM) {
+            const int cols = max(chunk_clamp_row(r1, a.total_rows) - row0, 0) * a.group;
+            if (s0 + lane < a.n_seq && cols <= a.col_split)
+                keys += (float)((cols + sum_qt - 1) / sum_qt) * (float)min(max(ctx, 0), a.max_blocks * a.block_size);
+        } else {
+            if (m != ~0ull) break;
+        }
     }
-    if (below == 0) return false;
-    t.seq = __builtin_amdgcn_readfirstlane(below - 1);
-    t.row0 = chunk_clamp_row(a.cu_seqlens[t.seq], a.total_rows);
-    t.rows = max(chunk_clamp_row(a.cu_seqlens[t.seq + 1], a.total_rows) - t.row0, 0);
+    if constexpr (SUM) {
+        *sum = as_float(__builtin_amdgcn_readfirstlane(as_u32(wave_sum(keys))));
+    }
+    if (t.seq < 0) return false;
     t.cols = t.rows * a.group;
     const int n_tiles = (t.cols + qt - 1) / qt;
-    const int tile = slot - (int)((int64_t)t.row0 * a.group / qt + t.seq);
+    const int tile = slot - (t.row0 * a.group / qt + t.seq);
     if (tile < 0 || tile >= n_tiles) return false;
     // causal: the tiles with the longest key loops start first
     t.col0 = (a.causal ? n_tiles - 1 - tile : tile) * qt;
-    t.ctx = min(max(a.ctx_lens[t.seq], 0), a.max_blocks * a.block_size);
     t.p0 = t.ctx - t.rows;
-    t.keys = a.causal ? max(t.p0 + (min(t.col0 + qt, t.cols) - 1) / a.group + 1, 0) : t.ctx;
+    t.keys = a.causal ? max(t.p0 + chunk_row_of(a, min(t.col0 + qt, t.cols) - 1) + 1, 0) : t.ctx;
     return true;
 }
 
-// Keys per range of a tile that can see `keys` keys, when up to z workgroups share it.
+// Keys per range of a tile that can see `keys` keys, when up to z workgroups share it: a range has `min_keys` keys or
+// more, a multiple of bn.
 __device__ __forceinline__ int chunk_range_keys(int keys, int z, int bn, int min_keys) {
     const int per = (keys + z - 1) / z;
     return max((per + bn - 1) / bn * bn, min_keys);
@@ -140,7 +161,23 @@ __device__ __forceinline__ void chunk_fill_outside(const ChunkArgs &a, int part,
 }
 
 constexpr int kChunkFillGroups = 8;    // workgroups of a grid that only look after rows outside every sequence
-constexpr int kChunkMinKeys = 256;     // a key range is not cut below this
+constexpr int kChunkMinKeys = 256;     // a key range is not cut below this (LDS kernel / narrow kernel)
+constexpr int kNarrowMinKeys = 256;
+constexpr int kNarrowStep = 128;       // keys that the four waves of a narrow workgroup take per turn
+
+// Least keys per range of the narrow kernel: the keys of all its tiles shared out evenly over the workgroups that the
+// chip holds at once (less one per tile, for the ranges that a tile ends with), so that a long context is cut into more
+// ranges than a short one and the workgroups end together.  Every wave computes it from the lengths; the merge reads it
+// from the workspace.
+__device__ __forceinline__ int narrow_min_keys(const ChunkArgs &a, float sum) {
+    const int per = __builtin_amdgcn_readfirstlane((int)fminf(sum * a.per_group, 1.0e9f));
+    return max((per / kNarrowStep + 1) * kNarrowStep, kNarrowMinKeys);
+}
+
+// A column's P = 2^((s - m) c) refers to a point m that need not be its maximum: O / l does not depend on it.  A lane's P
+// are positive, so a sum below kGuard bounds each of them, far from fp16's largest value.
+constexpr float kGuard = 4096.f;
+constexpr int kAnyColumns = 1 << 30;   // more columns than a call can have
 
 // ---- tiles through LDS --------------------------------------------------------------------------------------------
 // One workgroup (WAVES waves) owns 16 * QB * WAVES columns, each wave 16 * QB of them for the whole key loop.  Tiles
@@ -148,7 +185,7 @@ constexpr int kChunkMinKeys = 256;     // a key range is not cut below this
 // ahead: a table entry is never waited for), decoded into the other LDS buffer one tile ahead, and read by all waves.
 // ALIGN4: block_size % 4 == 0, so four keys from a multiple of four on share a block (one table lookup).
 template <int D, int MODE, int QB, int BN, int OCC, int WAVES, bool ALIGN4, bool ZS>
-__global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn_kernel(ChunkArgs a, int n_slots, int col_min) {
+__global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn_kernel(ChunkArgs a, int n_slots) {
     constexpr int DW = D / 4;
     constexpr bool BF8 = MODE == FEATHER_E5M2;
     constexpr int KS = BF8 ? (D + 16) / 2 : D + 8;   // K row pitch in LDS, in fp16 units (bf8: D + 16 bytes)
@@ -165,7 +202,7 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn_kernel(ChunkArgs a
     _Float16 *const lds = reinterpret_cast<_Float16 *>(smem);
     auto swz = [](int row) { return (row ^ (row >> 2)) & (CH - 1); };
 
-    const int work = n_slots * a.n_kv_heads * (ZS ? a.z : 1);
+    const int work = n_slots * a.n_kv_heads * (ZS ? a.z_wide : 1);
     int bid = blockIdx.x;
     if (bid >= work) {
         chunk_fill_outside<D>(a, bid - work, gridDim.x - work, kThreads);
@@ -174,17 +211,17 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn_kernel(ChunkArgs a
     if (work % 8 == 0) bid = (bid % 8) * (work / 8) + bid / 8;   // an XCD (own L2) works through neighbouring tiles of one KV head
     int zr = 0;
     if constexpr (ZS) {
-        zr = bid % a.z;
-        bid /= a.z;
+        zr = bid % a.z_wide;
+        bid /= a.z_wide;
     }
     const int kvh = bid / n_slots;
     ChunkTile t;
     if (!chunk_find_tile(a, bid % n_slots, QT, t)) return;
-    if (t.cols < col_min) return;                      // a short sequence: the other kernel's work
+    if (t.cols <= a.col_split) return;                 // a short run of rows: the other kernel's work
 
     int key_begin = 0, key_end = t.keys;
     if constexpr (ZS) {
-        const int per = chunk_range_keys(t.keys, a.z, BN, kChunkMinKeys);
+        const int per = chunk_range_keys(t.keys, a.z_wide, BN, kChunkMinKeys);
         key_begin = zr * per;
         key_end = min(t.keys, key_begin + per);
         if (key_begin >= key_end) return;              // the merge knows which ranges exist
@@ -201,13 +238,13 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn_kernel(ChunkArgs a
     int last[QB];
 #pragma unroll
     for (int b = 0; b < QB; b++) {
-        const int c = min(qc0 + 16 * b + j, t.cols - 1), r = c / a.group;
+        const int c = min(qc0 + 16 * b + j, t.cols - 1), r = chunk_row_of(a, c);
         item[b] = (int64_t)(t.row0 + r) * a.n_q_heads + kvh * a.group + (c - r * a.group);
         last[b] = a.causal ? t.p0 + r : t.ctx - 1;
     }
-    const int wave_first = a.causal ? t.p0 + min(qc0, t.cols - 1) / a.group : t.ctx - 1;     // smallest and largest last key of the wave
-    const int wave_last = a.causal ? t.p0 + min(qc0 + 16 * QB - 1, t.cols - 1) / a.group : t.ctx - 1;
-    const int tile_first = a.causal ? t.p0 + t.col0 / a.group : t.ctx - 1;
+    const int wave_first = a.causal ? t.p0 + chunk_row_of(a, min(qc0, t.cols - 1)) : t.ctx - 1;     // smallest and largest last key of the wave
+    const int wave_last = a.causal ? t.p0 + chunk_row_of(a, min(qc0 + 16 * QB - 1, t.cols - 1)) : t.ctx - 1;
+    const int tile_first = a.causal ? t.p0 + chunk_row_of(a, t.col0) : t.ctx - 1;
     const bool wave_has = qc0 < t.cols;
 
     half8_t qf[BF8 ? 1 : QB][BF8 ? 1 : STEPS];
@@ -461,7 +498,7 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn_kernel(ChunkArgs a
             const int64_t items = (int64_t)a.total_rows * a.n_q_heads, at = zr * items + item[b];
 #pragma unroll
             for (int d = 0; d < DB; d++) *reinterpret_cast<float4_t *>(a.part + at * D + 16 * d + 4 * kb) = o[b][d];
-            if (kb == 0) *reinterpret_cast<float2p_t *>(a.part + a.z * items * D + at * 2) = float2p_t{m_run[b], l};
+            if (kb == 0) *reinterpret_cast<float2p_t *>(a.part + a.z_wide * items * D + at * 2) = float2p_t{m_run[b], l};
         } else {
             const float inv = l == 0.f ? 0.f : 1.0f / l;          // no visible key: a zero result
 #pragma unroll
@@ -470,110 +507,593 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn_kernel(ChunkArgs a
     }
 }
 
-// Adds the key ranges of a column in range order; one thread per (row, head, four dims).  Rows of no sequence are
-// zeroed here (fill) or left alone.
+// ---- few columns: keys straight from the cache ----------------------------------------------------------------------
+// A drafted token or a handful of them: 16 * NB columns or fewer per (sequence, KV head), so the cache is read once and
+// its bytes bound the kernel.  One workgroup of four waves per (tile, KV head, key range); the waves take the range's
+// steps of 32 keys in turn, K and V go from memory to registers without LDS, NF steps in flight:
+//     S^T[key, col]   = K Q^T       a lane loads 16 codes of one key: the A operand of two products
+//     O_c^T[i, col]  += V_c^T P^T   dim = 4 i + c: the lane loads the same word of eight keys and byte c of them is the
+//                                   A operand of the c-th product, so V is transposed by the byte select of its decode
+// The block ids of a step are loaded NF steps before its rows are.  Each wave keeps its own reference point and sums;
+// they are joined through LDS, and the ranges by the merge kernel.
+__device__ __forceinline__ int64_t narrow_items(const ChunkArgs &a) {
+    return (a.narrow_rows ? (int64_t)a.n_seq * a.narrow_rows : a.total_rows) * a.n_q_heads;
+}
+__device__ __forceinline__ int64_t narrow_item(const ChunkArgs &a, int64_t item, int seq, int row0) {
+    return a.narrow_rows ? item + ((int64_t)seq * a.narrow_rows - row0) * a.n_q_heads : item;
+}
+
+template <int D, int MODE, int NB, bool POW2>
+__global__ __launch_bounds__(256, (D / 64) * NB <= 4 ? 2 : 1) void chunk_narrow_kernel(ChunkArgs a, int n_slots, int fill) {
+    constexpr int DW = D / 4, RB = D / 64, STEPS = D / 32, QT = 16 * NB, W = 4, STEP = 32;
+    constexpr bool BF8 = MODE == FEATHER_E5M2;
+    constexpr int NF = D == 64 ? (NB == 4 ? 2 : 4) : (D == 128 ? 2 : 1);
+    static_assert(STEP * W == kNarrowStep, "keys per turn");
+    __shared__ float ml_lds[NB][W][2][16];
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    float4_t *const x_lds = reinterpret_cast<float4_t *>(smem);     // [NB][W][RB * 4][64]
+
+    // Grid (sequence and KV head, key range, tile slot of the sequence).  Launch order, which goes round the XCDs: all
+    // sequences and KV heads of the first range, of the second, ..., and all that again for the second slot.  Slots and
+    // ranges that do not exist (a sequence has one slot more than it may need) then come last instead of falling on the
+    // same XCDs again and again.
+    const int zr = blockIdx.y;
+    if (fill && blockIdx.z == 0 && zr == 0) chunk_fill_outside<D>(a, blockIdx.x, gridDim.x, 256);
+    if (a.n_seq == 0) return;
+    const int seq_i = (int)(__umulhi(2u * blockIdx.x, a.kv_mul) >> a.kv_shift), kvh = blockIdx.x - seq_i * a.n_kv_heads;
+    const int slot = seq_i * gridDim.z + blockIdx.z;
+    // beside the LDS kernel every sequence of this one is a single tile: its slot is its number
+    const bool alone = a.col_split == kAnyColumns;
+    ChunkTile t;
+    int least = kNarrowMinKeys;
+    bool found;
+    if (a.z_narrow > 1) {
+        float sum;
+        found = chunk_find_tile<true>(a, slot, alone ? QT : kAnyColumns, t, QT, &sum);
+        least = narrow_min_keys(a, sum);
+        if (blockIdx.x + blockIdx.y + blockIdx.z == 0 && threadIdx.x == 0) *reinterpret_cast<int *>(a.part_narrow + narrow_items(a) * a.z_narrow * (D + 2)) = least;
+    } else {
+        found = chunk_find_tile(a, slot, alone ? QT : kAnyColumns, t);
+    }
+    if (!found || slot >= n_slots) return;
+    if (t.cols > a.col_split) return;                               // a long run of rows: the other kernel's work
+    const int per = chunk_range_keys(t.keys, a.z_narrow, kNarrowStep, least);
+    const int key_begin = zr * per, key_end = min(t.keys, key_begin + per);
+    if (key_begin >= key_end && (zr > 0 || a.z_narrow > 1)) return;  // the merge knows which ranges exist
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), j = lane & 15, kb = lane >> 4;
+    const int32_t *bt = a.block_tables + (int64_t)t.seq * a.max_blocks;
+    // address of a key's row: power-of-two blocks take a shift and a mask (and four keys from a multiple of four on are
+    // in one block), others the multiplication
+    const uint32_t block_bytes = (uint32_t)(a.n_kv_heads * a.block_size) * D;      // below 2^32: checked by the host
+    const int64_t head_bytes = (int64_t)kvh * a.block_size * D;
+    auto entry_of = [&](int pos) { return POW2 ? (uint32_t)pos >> a.div_shift : chunk_block_of(a, pos); };
+    auto slot_of = [&](int pos) { return POW2 ? (uint32_t)pos & (uint32_t)(a.block_size - 1) : (uint32_t)pos - chunk_block_of(a, pos) * (uint32_t)a.block_size; };
+    auto row_at = [&](const uint32_t *cache, int id, int pos, int byte) {
+        return reinterpret_cast<const char *>(cache) + head_bytes + ((uint64_t)min((uint32_t)id, a.max_blk) * block_bytes + (slot_of(pos) * D + byte));
+    };
+
+    struct Step {
+        u32x4 kw[2][RB];
+        uint32_t vw[RB][2][4];
+    };
+    struct Ids {
+        int k[2], v[2][POW2 ? 1 : 4];
+    };
+    Step steps[NF];
+    Ids ids[NF];
+    const int last_key = key_end - 1;                               // positions past the range repeat its last key and are masked
+    auto vpos = [&](int t0, int h, int r) { return POW2 ? (min(t0 + 16 * h + 4 * kb, last_key) & ~3) : min(t0 + 16 * h + 4 * kb + r, last_key); };
+    auto fetch_ids = [&](Ids &I, int t0) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            I.k[h] = bt[entry_of(min(t0 + 16 * h + j, last_key))];
+#pragma unroll
+            for (int r = 0; r < (POW2 ? 1 : 4); r++) I.v[h][r] = bt[entry_of(vpos(t0, h, r))];
+        }
+    };
+    auto load_step = [&](Step &S, const Ids &I, int t0) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const char *kr = row_at(a.k_cache, I.k[h], min(t0 + 16 * h + j, last_key), 16 * kb);
+#pragma unroll
+            for (int c = 0; c < RB; c++) S.kw[h][c] = *reinterpret_cast<const u32x4 *>(kr + 64 * c);
+            const char *vr = row_at(a.v_cache, I.v[h][0], vpos(t0, h, 0), 4 * j);
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                if constexpr (!POW2) vr = row_at(a.v_cache, I.v[h][r], vpos(t0, h, r), 4 * j);
+#pragma unroll
+                for (int c = 0; c < RB; c++) S.vw[c][h][r] = *reinterpret_cast<const uint32_t *>(vr + (POW2 ? r * D : 0) + 64 * c);
+            }
+        }
+    };
+    const int n_steps = (key_end - key_begin + STEP - 1) / STEP;
+    auto step_key = [&](int i) { return key_begin + STEP * (wave + W * i); };   // first key of the wave's i-th step
+    const int mine = n_steps > wave ? (n_steps - wave + W - 1) / W : 0;
+#pragma unroll
+    for (int f = 0; f < NF; f++)
+        if (f < mine) fetch_ids(ids[f], step_key(f));
+
+    // columns of this lane and their queries: k-slots of product st are dims 64 (st / 2) + 16 kb + 8 (st % 2) + {0..7}
+    int64_t item[NB];
+    int last[NB];
+    half8_t qf[BF8 ? 1 : NB][BF8 ? 1 : STEPS];
+    long qf8[BF8 ? NB : 1][BF8 ? STEPS : 1];
+    u32x2 qw[NB][STEPS];
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        const int c = min(t.col0 + 16 * b + j, t.cols - 1), r = chunk_row_of(a, c);
+        item[b] = (int64_t)(t.row0 + r) * a.n_q_heads + kvh * a.group + (c - r * a.group);
+        last[b] = a.causal ? t.p0 + r : t.ctx - 1;
+#pragma unroll
+        for (int st = 0; st < STEPS; st++)
+            qw[b][st] = *reinterpret_cast<const u32x2 *>(a.q + item[b] * DW + 16 * (st / 2) + 4 * kb + 2 * (st % 2));
+    }
+#pragma unroll
+    for (int f = 0; f < NF; f++)
+        if (f < mine) {
+            load_step(steps[f], ids[f], step_key(f));
+            if (f + NF < mine) fetch_ids(ids[f], step_key(f + NF));
+        }
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int st = 0; st < STEPS; st++) {
+            if constexpr (BF8) qf8[b][st] = __builtin_bit_cast(long, qw[b][st]);
+            else qf[b][st] = chunk_dec8<MODE>(qw[b][st].x, qw[b][st].y);
+        }
+    const int tile_first = a.causal ? t.p0 + chunk_row_of(a, t.col0) : t.ctx - 1;
+
+    float4_t o[NB][RB][4];
+    float m_run[NB], mc_run[NB], l_run[NB];   // reference point (raw, and times scale * log2 e), the lane's share of the sum
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        m_run[b] = mc_run[b] = -INFINITY;
+        l_run[b] = 0.f;
+#pragma unroll
+        for (int rb = 0; rb < RB; rb++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) o[b][rb][c] = float4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    auto compute_step = [&](Step &S, int t0) {
+        const bool masked = t0 + STEP - 1 > min(tile_first, last_key);   // some column does not see some key (wave-uniform)
+        bool nf = false;
+        if (BF8 && masked) {   // codes of inf and NaN must not meet the zero P of a column that does not see them
+            uint32_t any = 0;
+#pragma unroll
+            for (int c = 0; c < RB; c++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const uint32_t m = chunk_nonfinite(S.vw[c][h][r]);
+                        S.vw[c][h][r] &= ~m;
+                        any |= m;
+                    }
+            nf = __builtin_amdgcn_ballot_w64(any != 0) != 0;
+        }
+        half8_t p[NB];
+        float4_t sc[NB][2];
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int c = 0; c < RB; c++) {   // a key is decoded once for all column blocks
+                const float4_t zero = {0.f, 0.f, 0.f, 0.f};
+                if constexpr (BF8) {
+                    const long k0 = __builtin_bit_cast(long, u32x2{S.kw[h][c].x, S.kw[h][c].y}), k1 = __builtin_bit_cast(long, u32x2{S.kw[h][c].z, S.kw[h][c].w});
+#pragma unroll
+                    for (int b = 0; b < NB; b++) {
+                        sc[b][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf8_bf8(k0, qf8[b][2 * c], c == 0 ? zero : sc[b][h], 0, 0, 0);
+                        sc[b][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf8_bf8(k1, qf8[b][2 * c + 1], sc[b][h], 0, 0, 0);
+                    }
+                } else {
+                    const half8_t k0 = chunk_dec8<MODE>(S.kw[h][c].x, S.kw[h][c].y), k1 = chunk_dec8<MODE>(S.kw[h][c].z, S.kw[h][c].w);
+#pragma unroll
+                    for (int b = 0; b < NB; b++) {
+                        sc[b][h] = chunk_mfma16(k0, qf[b][2 * c], c == 0 ? zero : sc[b][h]);
+                        sc[b][h] = chunk_mfma16(k1, qf[b][2 * c + 1], sc[b][h]);
+                    }
+                }
+            }
+        if (masked) {
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                int rel = min(last[b], last_key) - t0 - 4 * kb;         // key 16 h + 4 kb + r is hidden if 16 h + r > rel
+                asm volatile("" : "+v"(rel));
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        if (16 * h + r > rel) sc[b][h][r] = -INFINITY;
+            }
+        }
+        // P against the column's current reference point; the lane's share of the sum, needed anyway, tells whether that
+        // was safe (see kGuard).  If not -- the first keys of a column, whose reference is -inf, or a score far above it --
+        // the references are raised to the true maxima, the accumulators rescaled and P computed again.
+        float sum[NB];
+        auto exp_block = [&](int b, float mc) {
+            uint32_t pw[4];
+            sum[b] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][i >> 1][2 * (i & 1)], a.scale_log2e, -mc));
+                const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][i >> 1][2 * (i & 1) + 1], a.scale_log2e, -mc));
+                pw[i] = as_u32(__builtin_convertvector(float2p_t{e0, e1}, half2_t));
+                sum[b] = dot2(pw[i], 0x3c003c00u, sum[b]);              // the sum takes the rounded values that multiply V
+            }
+            p[b] = __builtin_bit_cast(half8_t, u32x4{pw[0], pw[1], pw[2], pw[3]});
+        };
+        bool safe = true;
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            exp_block(b, mc_run[b]);
+            safe = safe && sum[b] < kGuard;
+        }
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(!safe) != 0, 0)) {
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const float4_t (&s)[2] = sc[b];
+                float mx = max3_raw(max3_raw(s[0][0], s[0][1], s[0][2]), s[0][3], s[1][0]);
+                mx = max_raw(max3_raw(mx, s[1][1], s[1][2]), s[1][3]);
+                mx = max_xor32(max_xor16(mx));
+                const float m_old = m_run[b], m_new = max_raw(m_old, mx);
+                // a column that has seen no key keeps the reference -inf: its scores are -inf here, its P zero
+                const float alpha = m_old == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_old - m_new) * a.scale_log2e);
+                m_run[b] = m_new;
+                mc_run[b] = m_new * a.scale_log2e;
+                l_run[b] *= alpha;
+#pragma unroll
+                for (int rb = 0; rb < RB; rb++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) o[b][rb][c] *= alpha;
+                exp_block(b, m_new == -INFINITY ? 0.f : mc_run[b]);
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < NB; b++) l_run[b] += sum[b];
+#pragma unroll
+        for (int rb = 0; rb < RB; rb++) {
+            uint32_t pr[4][4];   // [pair of keys][byte]
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+                    const uint32_t wa = S.vw[rb][h][2 * q], wb = S.vw[rb][h][2 * q + 1];
+                    uint32_t *out = pr[2 * h + q];
+                    if constexpr (BF8) {
+#pragma unroll
+                        for (int c = 0; c < 4; c++) out[c] = perm(wb, wa, 0x000c000cu | ((uint32_t)c << 8) | ((uint32_t)(4 + c) << 24));
+                    } else {   // codes of the two keys interleaved first: the decoder's pairs are then the key pairs
+                        dec_word<MODE>(perm(wb, wa, 0x05010400u), out[0], out[1]);
+                        dec_word<MODE>(perm(wb, wa, 0x07030602u), out[2], out[3]);
+                    }
+                }
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const half8_t vf = __builtin_bit_cast(half8_t, u32x4{pr[0][c], pr[1][c], pr[2][c], pr[3][c]});
+#pragma unroll
+                for (int b = 0; b < NB; b++) o[b][rb][c] = chunk_mfma16(vf, p[b], o[b][rb][c]);
+            }
+        }
+        if (BF8 && nf) {   // rare: what the zeros stand for, added for the columns that see the key
+            for (int key = t0; key <= min(t0 + STEP - 1, last_key); key++) {
+                const uint32_t *vr = reinterpret_cast<const uint32_t *>(row_at(a.v_cache, bt[entry_of(key)], key, 16 * kb));
+#pragma unroll
+                for (int rb = 0; rb < RB; rb++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const uint32_t w = vr[16 * rb + r], m = chunk_nonfinite(w);
+                        if (m != 0)
+#pragma unroll
+                            for (int c = 0; c < 4; c++)
+                                if ((m >> (8 * c)) & 1u) {
+                                    const float x = (float)__builtin_bit_cast(_Float16, (uint16_t)((w >> (8 * c)) << 8));
+#pragma unroll
+                                    for (int b = 0; b < NB; b++)
+                                        if (key <= last[b]) o[b][rb][c][r] += x;
+                                }
+                    }
+            }
+        }
+    };
+    for (int i = 0; i < mine; i += NF) {
+#pragma unroll
+        for (int f = 0; f < NF; f++) {
+            if (i + f < mine) {
+                compute_step(steps[f], step_key(i + f));
+                if (i + f + NF < mine) {
+                    load_step(steps[f], ids[f], step_key(i + f + NF));
+                    if (i + f + 2 * NF < mine) fetch_ids(ids[f], step_key(i + f + 2 * NF));
+                }
+            }
+        }
+    }
+
+    // ---- join the four waves: all partial results go to LDS, then W / NB waves finish a column block, a share of its
+    // dims each
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        float l = l_run[b];
+        l += __shfl_xor(l, 16, kWave);
+        l += __shfl_xor(l, 32, kWave);
+        if (kb == 0) {
+            ml_lds[b][wave][0][j] = m_run[b];
+            ml_lds[b][wave][1][j] = l;
+        }
+#pragma unroll
+        for (int rb = 0; rb < RB; rb++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)   // (rb, r): words 16 rb + 4 kb + r of the column
+                x_lds[((b * W + wave) * RB * 4 + rb * 4 + r) * 64 + lane] = float4_t{o[b][rb][0][r], o[b][rb][1][r], o[b][rb][2][r], o[b][rb][3][r]};
+    }
+    __syncthreads();
+    constexpr int SHARES = W / NB, UNITS = RB * 4 / SHARES;
+    const int b = wave / SHARES, u0 = (wave % SHARES) * UNITS;
+    const int col = t.col0 + 16 * b + j;
+    if (col >= t.cols) return;
+    float m = -INFINITY, wgt[W], sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; w++) m = fmaxf(m, ml_lds[b][w][0][j]);
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+        const float mw = ml_lds[b][w][0][j];
+        wgt[w] = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mw - m) * a.scale_log2e);
+        sum += wgt[w] * ml_lds[b][w][1][j];
+    }
+    const int row = chunk_row_of(a, col);
+    const int64_t it = (int64_t)(t.row0 + row) * a.n_q_heads + kvh * a.group + (col - row * a.group);
+    const int64_t items = narrow_items(a), at = zr * items + narrow_item(a, it, t.seq, t.row0);
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;                 // no visible key: a zero result
+#pragma unroll
+    for (int i = 0; i < UNITS; i++) {
+        const int u = u0 + i;
+        float4_t x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < W; w++)
+            if (wgt[w] != 0.f) x += x_lds[((b * W + w) * RB * 4 + u) * 64 + lane] * wgt[w];
+        const int w4 = 16 * (u >> 2) + 4 * kb + (u & 3);
+        if (a.z_narrow > 1) *reinterpret_cast<float4_t *>(a.part_narrow + at * D + 4 * w4) = x;
+        else chunk_store<D, MODE>(a, it, w4, sum == 0.f ? float4_t{0.f, 0.f, 0.f, 0.f} : x * inv);
+    }
+    if (a.z_narrow > 1 && u0 == 0 && kb == 0) *reinterpret_cast<float2p_t *>(a.part_narrow + a.z_narrow * items * D + at * 2) = float2p_t{m, sum};
+}
+
+// Adds the key ranges of a column in range order.  A workgroup holds 256 / (DW * zl) items (row, head); an item's dims
+// lie along DW threads, and zl of these rows of threads take the item's ranges in turn and are joined through LDS, so
+// that few items of many ranges are not one long chain of loads.  Rows of no sequence are zeroed here (fill) or left
+// alone; rows whose kernel had a single range have their result already.
+constexpr int kMergeSeqs = 1024;
+
 template <int D, int MODE>
-__global__ __launch_bounds__(256) void chunk_merge_kernel(ChunkArgs a, int qt, int bn) {
-    constexpr int DW = D / 4;
-    const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
+__global__ __launch_bounds__(256) void chunk_merge_kernel(ChunkArgs a, int qt_wide, int bn_wide, int qt_narrow, int zl) {
+    constexpr int DW = D / 4, G = 4;
+    __shared__ float4_t x_lds[256];
+    __shared__ float2p_t ml_lds[256];
+    __shared__ int cu_lds[kMergeSeqs + 1];
+    const bool cached = a.n_seq <= kMergeSeqs;         // the search for the row's sequence then is no chain of loads
+    if (cached)
+        for (int s = threadIdx.x; s <= a.n_seq; s += 256) cu_lds[s] = chunk_clamp_row(a.cu_seqlens[s], a.total_rows);
+    __syncthreads();
+    auto cu_at = [&](int s) { return cached ? cu_lds[s] : chunk_clamp_row(a.cu_seqlens[s], a.total_rows); };
+    const int tid = threadIdx.x, w4 = tid % DW, zi = (tid / DW) % zl;
     const int64_t items = (int64_t)a.total_rows * a.n_q_heads;
-    const int64_t item = gid / DW;
-    if (item >= items) return;
-    const int w4 = (int)(gid % DW), row = (int)(item / a.n_q_heads), head = (int)(item % a.n_q_heads);
-    int lo = 0, hi = a.n_seq;                          // last sequence that starts at or before the row
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (chunk_clamp_row(a.cu_seqlens[mid], a.total_rows) <= row) lo = mid; else hi = mid;
+    const int64_t item = (int64_t)blockIdx.x * (256 / (DW * zl)) + tid / (DW * zl);
+    int used = 0;
+    bool zero = false;
+    const float *part = a.part;                        // partial results of the row's kernel: [range][item][D], [range][item] pairs
+    int64_t part_items = items, part_item = item;
+    int z = 1;
+    if (item < items) {
+        const int row = (int)(item / a.n_q_heads), head = (int)(item % a.n_q_heads);
+        int lo = 0, hi = a.n_seq;                      // last sequence that starts at or before the row
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (cu_at(mid) <= row) lo = mid; else hi = mid;
+        }
+        const int r0 = cu_at(lo), r1 = max(cu_at(lo + 1), r0);
+        if (row < r0 || row >= r1) {
+            zero = a.fill;
+        } else {
+            const int ctx = min(max(a.ctx_lens[lo], 0), a.max_blocks * a.block_size), p0 = ctx - (r1 - r0);
+            const int cols = (r1 - r0) * a.group;
+            const bool narrow = cols <= a.col_split;
+            const int qt = narrow ? (a.narrow_rows ? kAnyColumns : qt_narrow) : qt_wide;
+            z = narrow ? a.z_narrow : a.z_wide;
+            const int col0 = ((row - r0) * a.group + head % a.group) / qt * qt;
+            const int keys = a.causal ? max(p0 + chunk_row_of(a, min(col0 + qt, cols) - 1) + 1, 0) : ctx;
+            if (z > 1) {
+                if (narrow) {
+                    part = a.part_narrow;
+                    part_items = narrow_items(a);
+                    part_item = narrow_item(a, item, lo, r0);
+                }
+                const int per = narrow ? chunk_range_keys(keys, z, kNarrowStep, *reinterpret_cast<const int *>(part + part_items * z * (D + 2)))
+                                       : chunk_range_keys(keys, z, bn_wide, kChunkMinKeys);
+                used = (keys + per - 1) / per;
+                zero = used == 0;
+            }
+        }
     }
-    const int r0 = chunk_clamp_row(a.cu_seqlens[lo], a.total_rows), r1 = max(chunk_clamp_row(a.cu_seqlens[lo + 1], a.total_rows), r0);
-    if (row < r0 || row >= r1) {
-        if (a.fill) chunk_store<D, MODE>(a, item, w4, float4_t{0.f, 0.f, 0.f, 0.f});
-        return;
-    }
-    const int ctx = min(max(a.ctx_lens[lo], 0), a.max_blocks * a.block_size), p0 = ctx - (r1 - r0);
-    const int cols = (r1 - r0) * a.group, col0 = ((row - r0) * a.group + head % a.group) / qt * qt;
-    const int keys = a.causal ? max(p0 + (min(col0 + qt, cols) - 1) / a.group + 1, 0) : ctx;
-    const int per = chunk_range_keys(keys, a.z, bn, kChunkMinKeys);
-    const int used = (keys + per - 1) / per;
-    const float2p_t *ml = reinterpret_cast<const float2p_t *>(a.part + a.z * items * D);
-    float m = -INFINITY;
-    for (int z = 0; z < used; z++) m = fmaxf(m, ml[z * items + item][0]);
+    const float2p_t *ml = reinterpret_cast<const float2p_t *>(part + z * part_items * D);
+    float m = -INFINITY, l = 0.f;
     float4_t acc = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.f;
-    for (int z = 0; z < used; z++) {
-        const float2p_t x = ml[z * items + item];
-        const float w = x[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((x[0] - m) * a.scale_log2e);
-        if (w == 0.f) continue;                        // a range of hidden keys only
-        acc += *reinterpret_cast<const float4_t *>(a.part + (z * items + item) * D + 4 * w4) * w;
-        l += x[1] * w;
+    for (int z0 = zi; z0 < used; z0 += G * zl) {       // G ranges per turn, all loads before the first use
+        float2p_t x[G];
+        float4_t y[G];
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            const int64_t at = min(z0 + g * zl, used - 1) * part_items + part_item;
+            x[g] = ml[at];
+            y[g] = *reinterpret_cast<const float4_t *>(part + at * D + 4 * w4);
+        }
+        float mg = m;
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            if (z0 + g * zl >= used) x[g] = float2p_t{-INFINITY, 0.f};
+            mg = fmaxf(mg, x[g][0]);
+        }
+        const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mg) * a.scale_log2e);
+        l *= keep;
+        acc *= keep;
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            if (x[g][0] == -INFINITY) continue;        // a range of hidden keys only
+            const float w = __builtin_amdgcn_exp2f((x[g][0] - mg) * a.scale_log2e);
+            l += x[g][1] * w;
+            acc += y[g] * w;
+        }
+        m = mg;
     }
-    chunk_store<D, MODE>(a, item, w4, l == 0.f ? float4_t{0.f, 0.f, 0.f, 0.f} : acc * (1.0f / l));
+    if (zl > 1) {
+        x_lds[tid] = acc;
+        ml_lds[tid] = float2p_t{m, l};
+        __syncthreads();
+        if (zi > 0) return;
+        float mg = m;
+        for (int k = 1; k < zl; k++) mg = fmaxf(mg, ml_lds[tid + k * DW][0]);
+        const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mg) * a.scale_log2e);
+        l *= keep;
+        acc *= keep;
+        for (int k = 1; k < zl; k++) {
+            const float2p_t x = ml_lds[tid + k * DW];
+            if (x[0] == -INFINITY) continue;
+            const float w = __builtin_amdgcn_exp2f((x[0] - mg) * a.scale_log2e);
+            l += x[1] * w;
+            acc += x_lds[tid + k * DW] * w;
+        }
+    }
+    if (used > 0 || zero) chunk_store<D, MODE>(a, item, w4, l == 0.f ? float4_t{0.f, 0.f, 0.f, 0.f} : acc * (1.0f / l));
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------
 
-struct ChunkShape { int qt, bn; };
+// How a call is cut: which kernels run, their tiles, and into how many key ranges.
+struct ChunkPlan {
+    bool wide, narrow;
+    int nb;                 // 16-column blocks of a narrow tile
+    int col_split;
+    int z_wide, z_narrow, narrow_rows;
+    float per_group;
+    int64_t wide_bytes, narrow_bytes;   // of the workspace, per range
+};
 
-static ChunkShape chunk_shape(int64_t d) {
-    switch (d) {
-        case 64: return {256, 64};
-        case 128: return {128, 64};
-        case 256: return {128, 64};
-        default: return {64, 32};
-    }
-}
+static int wide_columns(int64_t d) { return d == 64 ? 256 : (d == 512 ? 64 : 128); }
+static int narrow_most_blocks(int64_t d) { return d <= 128 ? 4 : (d == 256 ? 2 : 1); }
 
 static int64_t chunk_slots(int64_t total_rows, int64_t n_seq, int64_t group, int qt) { return total_rows * group / qt + n_seq; }
 
-// Workgroups that share a column tile: enough to give every CU two workgroups when the tiles alone do not.
-static int chunk_ranges(int64_t total_rows, int64_t n_seq, int64_t n_q_heads, int64_t n_kv_heads, int64_t d, int64_t max_ctx) {
-    const ChunkShape sh = chunk_shape(d);
-    const int64_t tiles = chunk_slots(total_rows, n_seq, n_q_heads / n_kv_heads, sh.qt) * n_kv_heads;
-    int64_t z = 512 / (tiles > 0 ? tiles : 1);
-    const int64_t most = (max_ctx + kChunkMinKeys - 1) / kChunkMinKeys;
+static int ranges_for(int64_t tiles, int64_t target, int64_t max_ctx, int64_t min_keys) {
+    int64_t z = target / (tiles > 0 ? tiles : 1);
+    const int64_t most = (max_ctx + min_keys - 1) / min_keys;
     if (z > most) z = most;
-    if (z > 64) z = 64;
+    if (z > 128) z = 128;
     return z < 1 ? 1 : (int)z;
 }
 
+static ChunkPlan chunk_plan(int64_t n_seq, int64_t total_rows, int64_t n_q_heads, int64_t n_kv_heads, int64_t d, int64_t max_ctx,
+                            int64_t max_q_len) {
+    ChunkPlan p;
+    const int64_t group = n_q_heads / n_kv_heads;
+    const int most = 16 * narrow_most_blocks(d);
+    const int64_t rows_most = max_q_len > 0 && max_q_len < total_rows ? max_q_len : total_rows;   // rows of the longest sequence, if the hint is right
+    const int64_t cols = rows_most * group;
+    const int64_t slots_each = n_seq > 0 ? (total_rows * group / 16 + n_seq) / n_seq : 1;
+    if (cols <= most && slots_each < 4096) {                 // all sequences are short (or the hint is wrong: more tiles each)
+        p.narrow = true;
+        p.wide = false;
+        p.col_split = kAnyColumns;
+        p.nb = cols <= 16 ? 1 : (cols <= 32 ? 2 : 4);
+    } else {
+        p.narrow = n_seq > 1 && rows_most * n_seq > total_rows;   // the lengths differ: some may be short
+        p.wide = true;
+        p.nb = narrow_most_blocks(d) >= 2 ? 2 : 1;
+        p.col_split = p.narrow ? 16 * p.nb : 0;
+    }
+    p.narrow_rows = p.wide && p.narrow ? (int)(p.col_split / group) : 0;
+    const int64_t each = n_seq > 0 ? (total_rows + n_seq - 1) / n_seq * group : 1;   // columns of a sequence of average length
+    p.z_wide = p.wide ? ranges_for((total_rows * group / wide_columns(d) + 1) * n_kv_heads, 512, max_ctx, kChunkMinKeys) : 1;
+    // the chip holds 256 workgroups of a kernel that fills a CU's registers, two or three times as many of a smaller one
+    const int weight = (int)(d / 64) * p.nb;
+    const int64_t groups = 256 * (weight <= 2 ? 3 : (weight <= 4 ? 2 : 1));
+    const int64_t tiles = (p.wide ? n_seq : n_seq * ((each + 16 * p.nb - 1) / (16 * p.nb))) * n_kv_heads;
+    // twice the even share, for contexts of different lengths
+    p.z_narrow = p.narrow && 2 * tiles <= groups ? ranges_for(tiles, 2 * groups, max_ctx, kNarrowMinKeys) : 1;
+    p.per_group = (float)n_kv_heads / (float)(groups - tiles > 0 ? groups - tiles : 1);
+    p.wide_bytes = total_rows * n_q_heads * (d + 2) * 4;
+    p.narrow_bytes = (p.narrow_rows ? n_seq * p.narrow_rows : total_rows) * n_q_heads * (d + 2) * 4;
+    return p;
+}
+
+static int64_t chunk_wide_scratch(const ChunkPlan &p) { return p.z_wide > 1 ? (p.z_wide * p.wide_bytes + 15) / 16 * 16 : 0; }
+static int64_t chunk_narrow_scratch(const ChunkPlan &p) { return p.z_narrow > 1 ? p.z_narrow * p.narrow_bytes + 16 : 0; }
+
 template <int D, int MODE, int QB, int BN, int OCC, int WAVES, bool ALIGN4, bool ZS>
-static int launch_chunk_kernel(const ChunkArgs &a, hipStream_t s) {
+static int launch_chunk_wide(const ChunkArgs &a, bool fill, hipStream_t s) {
     constexpr int QT = 16 * QB * WAVES;
     constexpr int KS = MODE == FEATHER_E5M2 ? (D + 16) / 2 : D + 8;
     constexpr size_t lds = (size_t)(BN * KS + D * BN) * 2 * 2;
     const char *me = "feather_paged_chunk_attn_fp8";
     const int64_t slots = chunk_slots(a.total_rows, a.n_seq, a.group, QT);
-    const int64_t blocks = slots * a.n_kv_heads * a.z;
+    const int64_t blocks = slots * a.n_kv_heads * a.z_wide;
     FEATHER_CHECK(blocks + kChunkFillGroups < (1ll << 31), FEATHER_ESHAPE, "%s: grid too large", me);
     auto kern = chunk_attn_kernel<D, MODE, QB, BN, OCC, WAVES, ALIGN4, ZS>;
     static unsigned long long lds_raised = 0;
     hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(kern), lds, lds_raised);
     FEATHER_CHECK(e == hipSuccess, FEATHER_ELAUNCH, "%s: cannot raise LDS limit: %s", me, hipGetErrorString(e));
-    hipLaunchKernelGGL(kern, dim3((unsigned)(blocks + (a.fill && !ZS ? kChunkFillGroups : 0))), dim3(64 * WAVES), lds, s, a, (int)slots, 0);
+    hipLaunchKernelGGL(kern, dim3((unsigned)(blocks + (fill ? kChunkFillGroups : 0))), dim3(64 * WAVES), lds, s, a, (int)slots);
     return check_launch(me);
 }
 
-template <int D, int MODE, int QB, int BN, int OCC, int WAVES>
-static int launch_chunk(const ChunkArgs &a, hipStream_t s) {
-    const bool al = a.block_size % 4 == 0;
-    if (a.z == 1)
-        return al ? launch_chunk_kernel<D, MODE, QB, BN, OCC, WAVES, true, false>(a, s)
-                  : launch_chunk_kernel<D, MODE, QB, BN, OCC, WAVES, false, false>(a, s);
-    const int rc = al ? launch_chunk_kernel<D, MODE, QB, BN, OCC, WAVES, true, true>(a, s)
-                      : launch_chunk_kernel<D, MODE, QB, BN, OCC, WAVES, false, true>(a, s);
-    if (rc != FEATHER_OK) return rc;
-    const int64_t threads = (int64_t)a.total_rows * a.n_q_heads * (D / 4);
-    hipLaunchKernelGGL((chunk_merge_kernel<D, MODE>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, a, 16 * QB * WAVES, BN);
+template <int D, int MODE, int NB, bool POW2>
+static int launch_chunk_narrow(const ChunkArgs &a, bool fill, hipStream_t s) {
+    constexpr size_t lds = (size_t)NB * 4 * (D / 64) * 4 * 64 * 16;
+    const char *me = "feather_paged_chunk_attn_fp8";
+    const int64_t slots = a.col_split < kAnyColumns ? a.n_seq : chunk_slots(a.total_rows, a.n_seq, a.group, 16 * NB);
+    const int64_t each = a.n_seq > 0 ? (slots + a.n_seq - 1) / a.n_seq : 1, pairs = a.n_seq > 0 ? (int64_t)a.n_seq * a.n_kv_heads : kChunkFillGroups;
+    FEATHER_CHECK(pairs < (1ll << 31) && each < 65536 && pairs * each * a.z_narrow < (1ll << 31), FEATHER_ESHAPE, "%s: grid too large", me);
+    auto kern = chunk_narrow_kernel<D, MODE, NB, POW2>;
+    static unsigned long long lds_raised = 0;
+    hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(kern), lds + 4096, lds_raised);
+    FEATHER_CHECK(e == hipSuccess, FEATHER_ELAUNCH, "%s: cannot raise LDS limit: %s", me, hipGetErrorString(e));
+    hipLaunchKernelGGL(kern, dim3((unsigned)pairs, (unsigned)a.z_narrow, (unsigned)each), dim3(256), lds, s, a, (int)slots, fill ? 1 : 0);
+    return check_launch(me);
+}
+
+template <int D, int MODE, bool POW2>
+static int launch_chunk(const ChunkArgs &a, const ChunkPlan &p, hipStream_t s) {
+    constexpr int QB = D == 64 ? 4 : (D == 128 ? 2 : 1), BN = D == 512 ? 32 : 64, OCC = D <= 128 ? 2 : 1, WAVES = D == 256 ? 8 : 4;
+    const bool merge = a.z_wide > 1 || a.z_narrow > 1;
+    bool fill = a.fill && !merge;                            // rows outside every sequence: the merge's work, or the first kernel's
+    int rc = FEATHER_OK;
+    if (p.wide) {
+        rc = a.z_wide > 1 ? launch_chunk_wide<D, MODE, QB, BN, OCC, WAVES, POW2, true>(a, fill, s)
+                          : launch_chunk_wide<D, MODE, QB, BN, OCC, WAVES, POW2, false>(a, fill, s);
+        fill = false;
+    }
+    if (rc == FEATHER_OK && p.narrow) {
+        if (p.nb == 1) rc = launch_chunk_narrow<D, MODE, 1, POW2>(a, fill, s);
+        if constexpr (D <= 256)
+            if (p.nb == 2) rc = launch_chunk_narrow<D, MODE, 2, POW2>(a, fill, s);
+        if constexpr (D <= 128)
+            if (p.nb == 4) rc = launch_chunk_narrow<D, MODE, 4, POW2>(a, fill, s);
+    }
+    if (rc != FEATHER_OK || !merge) return rc;
+    constexpr int DW = D / 4;
+    int zl = 1;                                              // four ranges per thread and turn; rows of the LDS kernel have few
+    while (!p.wide && zl * 4 < a.z_narrow && zl * DW < 256) zl *= 2;
+    const int64_t per_group = 256 / (DW * zl), items = (int64_t)a.total_rows * a.n_q_heads;
+    hipLaunchKernelGGL((chunk_merge_kernel<D, MODE>), dim3((unsigned)((items + per_group - 1) / per_group)), dim3(256), 0, s, a,
+                       16 * QB * WAVES, BN, 16 * p.nb, zl);
     return check_launch("feather_paged_chunk_attn_fp8 (merge of the key ranges)");
 }
 
-template <int MODE>
-static int dispatch_chunk(const ChunkArgs &a, int64_t d, hipStream_t s) {
+template <int MODE, bool POW2>
+static int dispatch_chunk(const ChunkArgs &a, const ChunkPlan &p, int64_t d, hipStream_t s) {
     switch (d) {
-        case 64: return launch_chunk<64, MODE, 4, 64, 2, 4>(a, s);
-        case 128: return launch_chunk<128, MODE, 2, 64, 2, 4>(a, s);
-        case 256: return launch_chunk<256, MODE, 1, 64, 1, 8>(a, s);
-        default: return launch_chunk<512, MODE, 1, 32, 1, 4>(a, s);
+        case 64: return launch_chunk<64, MODE, POW2>(a, p, s);
+        case 128: return launch_chunk<128, MODE, POW2>(a, p, s);
+        case 256: return launch_chunk<256, MODE, POW2>(a, p, s);
+        default: return launch_chunk<512, MODE, POW2>(a, p, s);
     }
 }
 
@@ -585,8 +1105,8 @@ extern "C" int64_t feather_paged_chunk_attn_scratch_bytes(int64_t n_seq, int64_t
                                                           int64_t n_kv_heads, int64_t d, int64_t max_ctx,
                                                           int64_t max_q_len) {
     if (n_seq <= 0 || total_rows <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || d <= 0 || max_ctx <= 0 || max_q_len < 0) return 0;
-    const int z = chunk_ranges(total_rows, n_seq, n_q_heads, n_kv_heads, d, max_ctx);
-    return z > 1 ? z * total_rows * n_q_heads * (d + 2) * 4 : 0;
+    const ChunkPlan p = chunk_plan(n_seq, total_rows, n_q_heads, n_kv_heads, d, max_ctx, max_q_len);
+    return chunk_wide_scratch(p) + chunk_narrow_scratch(p);
 }
 
 extern "C" int feather_paged_chunk_attn_fp8(const void *q, const void *k_cache, const void *v_cache, const void *block_tables,
@@ -616,8 +1136,9 @@ extern "C" int feather_paged_chunk_attn_fp8(const void *q, const void *k_cache, 
                       total_rows < (1ll << 30) && n_seq < (1ll << 30) && n_q_heads < (1ll << 20) &&
                       total_rows * n_q_heads < (1ll << 30),
                   FEATHER_ESHAPE, "%s: shape too large", me);
-    FEATHER_CHECK(n_blocks * n_kv_heads < (1ll << 32) && n_blocks * n_kv_heads * block_size < (1ll << 32), FEATHER_ESHAPE,
-                  "%s: the cache holds more than 2^32 rows", me);
+    FEATHER_CHECK(n_blocks * n_kv_heads < (1ll << 32) && n_blocks * n_kv_heads * block_size < (1ll << 32) &&
+                      n_kv_heads * block_size * d < (1ll << 31),
+                  FEATHER_ESHAPE, "%s: a cache of more than 2^32 rows, or a block of 2 GiB", me);
     if (total_rows == 0) return FEATHER_OK;
     if (n_seq == 0 && !fill) return FEATHER_OK;
     FEATHER_CHECK(q && k_cache && v_cache && out && cu_seqlens && (n_seq == 0 || (ctx_lens && (block_tables || max_blocks == 0))), FEATHER_EINVAL,
@@ -625,22 +1146,31 @@ extern "C" int feather_paged_chunk_attn_fp8(const void *q, const void *k_cache, 
     FEATHER_CHECK(aligned(q, 8) && aligned(k_cache, 16) && aligned(v_cache, 16) && aligned(out, 16) && aligned(scratch, 16) &&
                       aligned(block_tables, 4) && aligned(cu_seqlens, 4) && aligned(ctx_lens, 4),
                   FEATHER_EINVAL, "%s: misaligned pointer", me);
-    int z = n_seq > 0 ? chunk_ranges(total_rows, n_seq, n_q_heads, n_kv_heads, d, max_blocks * block_size) : 1;
-    if (!scratch) z = 1;
-    while (z > 1 && z * total_rows * n_q_heads * (d + 2) * 4 > scratch_bytes) z--;   // a smaller workspace: fewer ranges
-    int shift = 0;
-    while ((1ll << shift) < block_size) shift++;
+    ChunkPlan p = chunk_plan(n_seq, total_rows, n_q_heads, n_kv_heads, d, max_blocks * block_size, max_q_len);
+    const int64_t room = scratch && n_seq > 0 ? scratch_bytes : 0;   // a smaller workspace: fewer ranges
+    while (chunk_wide_scratch(p) > room) p.z_wide--;
+    while (chunk_wide_scratch(p) + chunk_narrow_scratch(p) > room) p.z_narrow--;
+    auto divisor = [](int64_t size, uint32_t &mul, int &shift) {   // see ChunkArgs
+        shift = 0;
+        while ((1ll << shift) < size) shift++;
+        mul = (uint32_t)((1ull << (31 + shift)) / (uint64_t)size + 1);
+    };
     ChunkArgs a;
+    divisor(block_size, a.div_mul, a.div_shift);
+    divisor(n_q_heads / n_kv_heads, a.group_mul, a.group_shift);
+    divisor(n_kv_heads, a.kv_mul, a.kv_shift);
     a.q = (const uint32_t *)q; a.k_cache = (const uint32_t *)k_cache; a.v_cache = (const uint32_t *)v_cache;
     a.block_tables = (const int32_t *)block_tables; a.cu_seqlens = (const int32_t *)cu_seqlens; a.ctx_lens = (const int32_t *)ctx_lens;
     a.out = out; a.part = (float *)scratch;
     a.n_seq = (int)n_seq; a.total_rows = (int)total_rows; a.n_q_heads = (int)n_q_heads; a.n_kv_heads = (int)n_kv_heads;
     a.group = (int)(n_q_heads / n_kv_heads); a.block_size = (int)block_size; a.max_blocks = (int)max_blocks;
     a.max_blk = (uint32_t)(n_blocks - 1);
-    a.div_mul = (uint32_t)((1ull << (31 + shift)) / (uint64_t)block_size + 1);
-    a.div_shift = shift;
-    a.causal = causal; a.z = z; a.out_kind = out_kind; a.fill = fill;
+    a.causal = causal; a.out_kind = out_kind; a.fill = fill;
+    a.z_wide = p.z_wide; a.z_narrow = p.z_narrow; a.per_group = p.per_group; a.narrow_rows = p.narrow_rows;
+    a.part_narrow = reinterpret_cast<float *>(static_cast<char *>(scratch) + chunk_wide_scratch(p)); a.col_split = p.col_split;
     a.scale_log2e = scale * 1.4426950408889634f;
-    return mode == FEATHER_E5M2 ? dispatch_chunk<FEATHER_E5M2>(a, d, (hipStream_t)stream)
-                                : dispatch_chunk<FEATHER_E4M3>(a, d, (hipStream_t)stream);
+    hipStream_t s = (hipStream_t)stream;
+    const bool al = block_size % 4 == 0 && (block_size & (block_size - 1)) == 0;
+    if (mode == FEATHER_E5M2) return al ? dispatch_chunk<FEATHER_E5M2, true>(a, p, d, s) : dispatch_chunk<FEATHER_E5M2, false>(a, p, d, s);
+    return al ? dispatch_chunk<FEATHER_E4M3, true>(a, p, d, s) : dispatch_chunk<FEATHER_E4M3, false>(a, p, d, s);
 }

@@ -268,7 +268,7 @@ def test_workspace_small_or_missing(dev, orc):
     need = L.feather_paged_chunk_attn_scratch_bytes(2, 8, 8, 2, 64, mb * 16, 0)
     assert need > 0
     per = 8 * 8 * 66 * 4
-    for size in (0, per - 1, per, 2 * per, need):
+    for size in (0, per - 1, per, 2 * per, 2 * per + 16, 3 * per + 16, need):
         ws = torch.empty(max(size, 16), dtype=torch.uint8, device=dev)
         out = torch.full((8, 8, 64), float("nan"), device=dev)
         N.check(L.feather_paged_chunk_attn_fp8(*[x.data_ptr() for x in t], out.data_ptr(), N.CHUNK_OUT_F32, 0,

@@ -32,8 +32,13 @@ def test_chunk_attention_argument_checks():
     size = L.feather_paged_chunk_attn_scratch_bytes
     assert size(0, 4, 8, 4, 64, 100, 0) == 0 and size(1, 4, 8, 4, 64, 100, 0) == 0 and size(-1, 4, 8, 4, 64, 100, 0) == 0
     z, rest = divmod(size(1, 4, 8, 4, 64, 100000, 4), 4 * 8 * 66 * 4)      # whole ranges of (d + 2) floats per row and head
-    assert rest == 0 and z > 1
-    assert size(8, 1 << 20, 8, 4, 64, 100000, 0) == 0                       # enough tiles to fill the chip
+    assert rest == 16 and z > 1
+    assert size(1, 1 << 20, 8, 4, 64, 100000, 0) == 0                       # enough tiles to fill the chip
+    for n_seq in (1, 3, 100, 5000):                                         # never out of proportion, whatever the lengths
+        for rows in (n_seq, 10 * n_seq, 1000 * n_seq, 1 << 20):
+            for d in (64, 128, 256, 512):
+                for hint in (0, 1, 64, rows):
+                    assert size(n_seq, rows, 32, 4, d, 1 << 20, hint) < 1 << 30
 
 
 def test_rope_chunk_argument_checks():
