@@ -60,11 +60,16 @@ __device__ __forceinline__ int chunk_clamp_row(int r, int total) { return min(ma
 
 __device__ __forceinline__ int chunk_row_of(const ChunkArgs &a, int col) { return (int)(__umulhi(2u * (uint32_t)col, a.group_mul) >> a.group_shift); }
 
-template <bool SUM = false>
-__device__ __forceinline__ bool chunk_find_tile(const ChunkArgs &a, int slot, int qt, ChunkTile &t, int sum_qt = 1, float *sum = nullptr) {
+// sequence s, its tile from column col0 on
+__device__ __forceinline__ void chunk_tile_at(const ChunkArgs &a, int col0, int qt, ChunkTile &t) {
+    t.col0 = col0;
+    t.p0 = t.ctx - t.rows;
+    t.keys = a.causal ? max(t.p0 + chunk_row_of(a, min(t.col0 + qt, t.cols) - 1) + 1, 0) : t.ctx;
+}
+
+__device__ __forceinline__ bool chunk_find_tile(const ChunkArgs &a, int slot, int qt, ChunkTile &t) {
     const int lane = lane_id();
     t.seq = -1;
-    float keys = 0.f;       // SUM: the lane's share of the keys of all tiles of sum_qt columns (an estimate will do)
     for (int s0 = 0; s0 < a.n_seq; s0 += kWave) {
         const int s = min(s0 + lane, a.n_seq - 1);
         const int r0 = a.cu_seqlens[s], r1 = a.cu_seqlens[s + 1], ctx = a.ctx_lens[s];
@@ -77,26 +82,14 @@ __device__ __forceinline__ bool chunk_find_tile(const ChunkArgs &a, int slot, in
             t.rows = max(chunk_clamp_row(__builtin_amdgcn_readlane(r1, at), a.total_rows) - t.row0, 0);
             t.ctx = min(max(__builtin_amdgcn_readlane(ctx, at), 0), a.max_blocks * a.block_size);
         }
-        if constexpr (SUM) {
-            const int cols = max(chunk_clamp_row(r1, a.total_rows) - row0, 0) * a.group;
-            if (s0 + lane < a.n_seq && cols <= a.col_split)
-                keys += (float)((cols + sum_qt - 1) / sum_qt) * (float)min(max(ctx, 0), a.max_blocks * a.block_size);
-        } else {
-            if (m != ~0ull) break;
-        }
-    }
-    if constexpr (SUM) {
-        *sum = as_float(__builtin_amdgcn_readfirstlane(as_u32(wave_sum(keys))));
+        if (m != ~0ull) break;
     }
     if (t.seq < 0) return false;
     t.cols = t.rows * a.group;
     const int n_tiles = (t.cols + qt - 1) / qt;
     const int tile = slot - (t.row0 * a.group / qt + t.seq);
     if (tile < 0 || tile >= n_tiles) return false;
-    // causal: the tiles with the longest key loops start first
-    t.col0 = (a.causal ? n_tiles - 1 - tile : tile) * qt;
-    t.p0 = t.ctx - t.rows;
-    t.keys = a.causal ? max(t.p0 + chunk_row_of(a, min(t.col0 + qt, t.cols) - 1) + 1, 0) : t.ctx;
+    chunk_tile_at(a, (a.causal ? n_tiles - 1 - tile : tile) * qt, qt, t);   // causal: the tiles with the longest key loops start first
     return true;
 }
 
@@ -169,7 +162,14 @@ constexpr int kNarrowStep = 128;       // keys that the four waves of a narrow w
 // chip holds at once (less one per tile, for the ranges that a tile ends with), so that a long context is cut into more
 // ranges than a short one and the workgroups end together.  Every wave computes it from the lengths; the merge reads it
 // from the workspace.
-__device__ __forceinline__ int narrow_min_keys(const ChunkArgs &a, float sum) {
+__device__ __forceinline__ int narrow_min_keys(const ChunkArgs &a, int qt) {
+    float keys = 0.f;       // an estimate will do
+    for (int s = lane_id(); s < a.n_seq; s += kWave) {
+        const int rows = max(chunk_clamp_row(a.cu_seqlens[s + 1], a.total_rows) - chunk_clamp_row(a.cu_seqlens[s], a.total_rows), 0);
+        const int cols = rows * a.group;
+        if (cols <= a.col_split) keys += (float)((cols + qt - 1) / qt) * (float)min(max(a.ctx_lens[s], 0), a.max_blocks * a.block_size);
+    }
+    const float sum = as_float(__builtin_amdgcn_readfirstlane(as_u32(wave_sum(keys))));
     const int per = __builtin_amdgcn_readfirstlane((int)fminf(sum * a.per_group, 1.0e9f));
     return max((per / kNarrowStep + 1) * kNarrowStep, kNarrowMinKeys);
 }
@@ -510,12 +510,55 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn_kernel(ChunkArgs a
 // ---- few columns: keys straight from the cache ----------------------------------------------------------------------
 // A drafted token or a handful of them: 16 * NB columns or fewer per (sequence, KV head), so the cache is read once and
 // its bytes bound the kernel.  One workgroup of four waves per (tile, KV head, key range); the waves take the range's
-// steps of 32 keys in turn, K and V go from memory to registers without LDS, NF steps in flight:
-//     S^T[key, col]   = K Q^T       a lane loads 16 codes of one key: the A operand of two products
-//     O_c^T[i, col]  += V_c^T P^T   dim = 4 i + c: the lane loads the same word of eight keys and byte c of them is the
+// steps of 32 keys in turn and share nothing until the end:
+//     S^T[key, col]   = K Q^T       a lane holds 16 codes of one key: the A operand of two products
+//     O_c^T[i, col]  += V_c^T P^T   dim = 4 i + c: the lane holds the same word of eight keys and byte c of them is the
 //                                   A operand of the c-th product, so V is transposed by the byte select of its decode
-// The block ids of a step are loaded NF steps before its rows are.  Each wave keeps its own reference point and sums;
-// they are joined through LDS, and the ranges by the merge kernel.
+// RING > 0 (block_size a multiple of 16, so 16 keys from a multiple of 16 on are in one block): the packed rows go from
+// memory to LDS without passing through registers, RING steps of a wave in flight or in use, into a ring of the wave's
+// own (no barrier, only the wave's count of outstanding loads).  A load moves 1 KiB with a wave-uniform base -- the block
+// id is a scalar load, the address scalar arithmetic -- and the lane's constant offset.  Registers then hold one step
+// only, which is what lets NB = 4 at D = 128 keep enough bytes in flight.
+// RING = 0 (any block size): rows go to registers, NF steps in flight, an address for every key.
+// Each wave keeps its own reference point and sums; they are joined through LDS, and the ranges by the merge kernel.
+template <int D>
+struct NarrowStep {
+    u32x4 kw[2][D / 64];
+    uint32_t vw[D / 64][2][4];
+};
+
+typedef __attribute__((address_space(3))) unsigned char lds_byte;
+typedef __attribute__((address_space(1))) unsigned char global_byte;
+
+// K and V of a step from the wave's ring slot.  The reads are asm statements with their wait inside: the compiler does
+// not see that they read what the direct loads wrote (it would wait for all of those, not for the step's); the caller
+// waits for the step's loads.  A row of D bytes has its 16-byte chunks XORed with row bits, so that the rows a read
+// touches fall on different banks.
+template <int D>
+__device__ __forceinline__ int ring_swizzle(int row) { return D == 64 ? (row >> 1) & 3 : row & 7; }
+
+#define RING_V_OUT(c)                                                                                                   \
+    "=&v"(S.vw[c][0][0]), "=&v"(S.vw[c][0][1]), "=&v"(S.vw[c][0][2]), "=&v"(S.vw[c][0][3]), "=&v"(S.vw[c][1][0]),      \
+        "=&v"(S.vw[c][1][1]), "=&v"(S.vw[c][1][2]), "=&v"(S.vw[c][1][3])
+
+template <int D>
+__device__ __forceinline__ void ring_read(uint32_t slot, uint32_t koff, const uint32_t (&voff)[4], NarrowStep<D> &S) {
+    // chunk 4 c + kb of a row: the XOR leaves bits above the swizzle alone, so c moves the address by an XOR of 64 c
+#pragma unroll
+    for (int c = 0; c < D / 64; c++) {
+        const uint32_t x = 64u * c, k0 = slot + (koff ^ x), v0 = slot + (voff[0] ^ x), v1 = slot + (voff[1] ^ x),
+                       v2 = slot + (voff[2] ^ x), v3 = slot + (voff[3] ^ x);
+        asm volatile("ds_read_b128 %0, %10\n\tds_read_b128 %1, %10 offset:%15\n\t"
+                     "ds_read_b32 %2, %11 offset:%16\n\tds_read_b32 %3, %12 offset:%16\n\t"
+                     "ds_read_b32 %4, %13 offset:%16\n\tds_read_b32 %5, %14 offset:%16\n\t"
+                     "ds_read_b32 %6, %11 offset:%17\n\tds_read_b32 %7, %12 offset:%17\n\t"
+                     "ds_read_b32 %8, %13 offset:%17\n\tds_read_b32 %9, %14 offset:%17\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(S.kw[0][c]), "=&v"(S.kw[1][c]), RING_V_OUT(c)
+                     : "v"(k0), "v"(v0), "v"(v1), "v"(v2), "v"(v3), "n"(16 * D), "n"(32 * D), "n"(48 * D) : "memory");
+    }
+}
+#undef RING_V_OUT
+
 __device__ __forceinline__ int64_t narrow_items(const ChunkArgs &a) {
     return (a.narrow_rows ? (int64_t)a.n_seq * a.narrow_rows : a.total_rows) * a.n_q_heads;
 }
@@ -523,73 +566,64 @@ __device__ __forceinline__ int64_t narrow_item(const ChunkArgs &a, int64_t item,
     return a.narrow_rows ? item + ((int64_t)seq * a.narrow_rows - row0) * a.n_q_heads : item;
 }
 
-template <int D, int MODE, int NB, bool POW2>
-__global__ __launch_bounds__(256, (D / 64) * NB <= 4 ? 2 : 1) void chunk_narrow_kernel(ChunkArgs a, int n_slots, int fill) {
+template <int D, int MODE, int NB, int RING>
+__global__ __launch_bounds__(256, (D / 64) * NB <= 4 ? 2 : 1) void chunk_narrow_kernel(ChunkArgs a, int fill) {
     constexpr int DW = D / 4, RB = D / 64, STEPS = D / 32, QT = 16 * NB, W = 4, STEP = 32;
     constexpr bool BF8 = MODE == FEATHER_E5M2;
-    constexpr int NF = D == 64 ? (NB == 4 ? 2 : 4) : (D == 128 ? 2 : 1);
+    constexpr int NF = RING > 0 ? 1 : (D == 64 ? (NB == 4 ? 2 : 4) : (D == 128 ? 2 : 1));
     static_assert(STEP * W == kNarrowStep, "keys per turn");
     __shared__ float ml_lds[NB][W][2][16];
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     float4_t *const x_lds = reinterpret_cast<float4_t *>(smem);     // [NB][W][RB * 4][64]
 
-    // Grid (sequence and KV head, key range, tile slot of the sequence).  Launch order, which goes round the XCDs: all
-    // sequences and KV heads of the first range, of the second, ..., and all that again for the second slot.  Slots and
-    // ranges that do not exist (a sequence has one slot more than it may need) then come last instead of falling on the
-    // same XCDs again and again.
+    // Grid (sequence and KV head, key range).  In launch order, which goes round the XCDs, all first ranges come before all
+    // second ones and so on: ranges that do not exist come last.  A sequence has one tile here -- unless the caller's
+    // bound of its rows was wrong, then the workgroup takes its tiles one after the other.
     const int zr = blockIdx.y;
-    if (fill && blockIdx.z == 0 && zr == 0) chunk_fill_outside<D>(a, blockIdx.x, gridDim.x, 256);
+    if (fill && zr == 0) chunk_fill_outside<D>(a, blockIdx.x, gridDim.x, 256);
     if (a.n_seq == 0) return;
     const int seq_i = (int)(__umulhi(2u * blockIdx.x, a.kv_mul) >> a.kv_shift), kvh = blockIdx.x - seq_i * a.n_kv_heads;
-    const int slot = seq_i * gridDim.z + blockIdx.z;
-    // beside the LDS kernel every sequence of this one is a single tile: its slot is its number
-    const bool alone = a.col_split == kAnyColumns;
     ChunkTile t;
+    t.seq = seq_i;
+    t.row0 = chunk_clamp_row(a.cu_seqlens[seq_i], a.total_rows);
+    t.rows = max(chunk_clamp_row(a.cu_seqlens[seq_i + 1], a.total_rows) - t.row0, 0);
+    t.cols = t.rows * a.group;
+    t.ctx = min(max(a.ctx_lens[seq_i], 0), a.max_blocks * a.block_size);
     int least = kNarrowMinKeys;
-    bool found;
     if (a.z_narrow > 1) {
-        float sum;
-        found = chunk_find_tile<true>(a, slot, alone ? QT : kAnyColumns, t, QT, &sum);
-        least = narrow_min_keys(a, sum);
-        if (blockIdx.x + blockIdx.y + blockIdx.z == 0 && threadIdx.x == 0) *reinterpret_cast<int *>(a.part_narrow + narrow_items(a) * a.z_narrow * (D + 2)) = least;
-    } else {
-        found = chunk_find_tile(a, slot, alone ? QT : kAnyColumns, t);
+        least = narrow_min_keys(a, QT);
+        if (blockIdx.x + blockIdx.y == 0 && threadIdx.x == 0) *reinterpret_cast<int *>(a.part_narrow + narrow_items(a) * a.z_narrow * (D + 2)) = least;
     }
-    if (!found || slot >= n_slots) return;
     if (t.cols > a.col_split) return;                               // a long run of rows: the other kernel's work
+#pragma nounroll
+    for (int col0 = 0; col0 < t.cols; col0 += QT) {
+    chunk_tile_at(a, col0, QT, t);
     const int per = chunk_range_keys(t.keys, a.z_narrow, kNarrowStep, least);
     const int key_begin = zr * per, key_end = min(t.keys, key_begin + per);
-    if (key_begin >= key_end && (zr > 0 || a.z_narrow > 1)) return;  // the merge knows which ranges exist
+    if (key_begin >= key_end && (zr > 0 || a.z_narrow > 1)) continue;   // the merge knows which ranges exist
 
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), j = lane & 15, kb = lane >> 4;
     const int32_t *bt = a.block_tables + (int64_t)t.seq * a.max_blocks;
-    // address of a key's row: power-of-two blocks take a shift and a mask (and four keys from a multiple of four on are
-    // in one block), others the multiplication
-    const uint32_t block_bytes = (uint32_t)(a.n_kv_heads * a.block_size) * D;      // below 2^32: checked by the host
+    const uint32_t block_bytes = (uint32_t)(a.n_kv_heads * a.block_size) * D;      // below 2^31: checked by the host
     const int64_t head_bytes = (int64_t)kvh * a.block_size * D;
-    auto entry_of = [&](int pos) { return POW2 ? (uint32_t)pos >> a.div_shift : chunk_block_of(a, pos); };
-    auto slot_of = [&](int pos) { return POW2 ? (uint32_t)pos & (uint32_t)(a.block_size - 1) : (uint32_t)pos - chunk_block_of(a, pos) * (uint32_t)a.block_size; };
+    auto slot_of = [&](int pos) { return (uint32_t)pos - chunk_block_of(a, pos) * (uint32_t)a.block_size; };
     auto row_at = [&](const uint32_t *cache, int id, int pos, int byte) {
         return reinterpret_cast<const char *>(cache) + head_bytes + ((uint64_t)min((uint32_t)id, a.max_blk) * block_bytes + (slot_of(pos) * D + byte));
     };
 
-    struct Step {
-        u32x4 kw[2][RB];
-        uint32_t vw[RB][2][4];
-    };
+    using Step = NarrowStep<D>;
     struct Ids {
-        int k[2], v[2][POW2 ? 1 : 4];
+        int k[2], v[2][4];
     };
     Step steps[NF];
     Ids ids[NF];
-    const int last_key = key_end - 1;                               // positions past the range repeat its last key and are masked
-    auto vpos = [&](int t0, int h, int r) { return POW2 ? (min(t0 + 16 * h + 4 * kb, last_key) & ~3) : min(t0 + 16 * h + 4 * kb + r, last_key); };
+    const int last_key = key_end - 1;                               // positions past the range repeat its last key (or its neighbours) and are masked
     auto fetch_ids = [&](Ids &I, int t0) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            I.k[h] = bt[entry_of(min(t0 + 16 * h + j, last_key))];
+            I.k[h] = bt[chunk_block_of(a, min(t0 + 16 * h + j, last_key))];
 #pragma unroll
-            for (int r = 0; r < (POW2 ? 1 : 4); r++) I.v[h][r] = bt[entry_of(vpos(t0, h, r))];
+            for (int r = 0; r < 4; r++) I.v[h][r] = bt[chunk_block_of(a, min(t0 + 16 * h + 4 * kb + r, last_key))];
         }
     };
     auto load_step = [&](Step &S, const Ids &I, int t0) {
@@ -598,21 +632,61 @@ __global__ __launch_bounds__(256, (D / 64) * NB <= 4 ? 2 : 1) void chunk_narrow_
             const char *kr = row_at(a.k_cache, I.k[h], min(t0 + 16 * h + j, last_key), 16 * kb);
 #pragma unroll
             for (int c = 0; c < RB; c++) S.kw[h][c] = *reinterpret_cast<const u32x4 *>(kr + 64 * c);
-            const char *vr = row_at(a.v_cache, I.v[h][0], vpos(t0, h, 0), 4 * j);
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                if constexpr (!POW2) vr = row_at(a.v_cache, I.v[h][r], vpos(t0, h, r), 4 * j);
+                const char *vr = row_at(a.v_cache, I.v[h][r], min(t0 + 16 * h + 4 * kb + r, last_key), 4 * j);
 #pragma unroll
-                for (int c = 0; c < RB; c++) S.vw[c][h][r] = *reinterpret_cast<const uint32_t *>(vr + (POW2 ? r * D : 0) + 64 * c);
+                for (int c = 0; c < RB; c++) S.vw[c][h][r] = *reinterpret_cast<const uint32_t *>(vr + 64 * c);
+            }
+        }
+    };
+    // RING: the wave's slots, 32 rows of K and 32 rows of V each
+    constexpr uint32_t kSlotBytes = 64 * D;
+    constexpr int kRowsPerLoad = 1024 / D, kLoadsPer16 = 16 / kRowsPerLoad, kDma = D / 16;
+    lds_byte *const ring = (lds_byte *)smem + wave * (RING > 0 ? RING : 1) * kSlotBytes;
+    const uint32_t ring_base = (uint32_t)(uintptr_t)ring;
+    uint32_t koff = 0, voff[4] = {0, 0, 0, 0}, lane_off[kLoadsPer16];
+    if constexpr (RING > 0) {
+        koff = j * D + 16 * (kb ^ ring_swizzle<D>(j));
+#pragma unroll
+        for (int r = 0; r < 4; r++) voff[r] = (4 * kb + r) * D + 16 * ((j >> 2) ^ ring_swizzle<D>(4 * kb + r)) + 4 * (j & 3);
+#pragma unroll
+        for (int q = 0; q < kLoadsPer16; q++) {                     // lane's byte inside 16 rows of a block, for the q-th load of them
+            const int row = q * kRowsPerLoad + lane / (D / 16), chunk = lane % (D / 16);
+            lane_off[q] = row * D + 16 * (chunk ^ ring_swizzle<D>(row));
+        }
+    }
+    const __attribute__((address_space(4))) int32_t *bt_const = (const __attribute__((address_space(4))) int32_t *)bt;   // read only while the kernel runs: scalar loads
+    auto group_id = [&](int t0, int h) { return bt_const[chunk_block_of(a, min(t0 + 16 * h, last_key & ~15))]; };
+    auto dma_step = [&](uint32_t slot, const int (&id)[2], int t0) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int pos = min(t0 + 16 * h, last_key & ~15);
+            const uint64_t off = (uint64_t)min((uint32_t)id[h], a.max_blk) * block_bytes + (uint64_t)head_bytes + slot_of(pos) * D;
+#pragma unroll
+            for (int which = 0; which < 2; which++) {
+                const char *base = reinterpret_cast<const char *>(which ? a.v_cache : a.k_cache) + off;
+#pragma unroll
+                for (int q = 0; q < kLoadsPer16; q++)
+                    __builtin_amdgcn_global_load_lds((const global_byte *)(base + lane_off[q]),
+                                                     (lds_byte *)(uintptr_t)(slot + (uint32_t)((which * 32 + 16 * h) * D + q * 1024)), 16, 0, 0);
             }
         }
     };
     const int n_steps = (key_end - key_begin + STEP - 1) / STEP;
     auto step_key = [&](int i) { return key_begin + STEP * (wave + W * i); };   // first key of the wave's i-th step
     const int mine = n_steps > wave ? (n_steps - wave + W - 1) / W : 0;
+    int gid[RING > 0 ? RING : 1][2];
+    if constexpr (RING == 0) {
 #pragma unroll
-    for (int f = 0; f < NF; f++)
-        if (f < mine) fetch_ids(ids[f], step_key(f));
+        for (int f = 0; f < NF; f++)
+            if (f < mine) fetch_ids(ids[f], step_key(f));
+    } else {
+#pragma unroll
+        for (int f = 0; f < RING; f++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) gid[f][h] = f < mine ? group_id(step_key(f), h) : 0;
+    }
 
     // columns of this lane and their queries: k-slots of product st are dims 64 (st / 2) + 16 kb + 8 (st % 2) + {0..7}
     int64_t item[NB];
@@ -629,12 +703,22 @@ __global__ __launch_bounds__(256, (D / 64) * NB <= 4 ? 2 : 1) void chunk_narrow_
         for (int st = 0; st < STEPS; st++)
             qw[b][st] = *reinterpret_cast<const u32x2 *>(a.q + item[b] * DW + 16 * (st / 2) + 4 * kb + 2 * (st % 2));
     }
+    int next_id[2] = {0, 0};
+    if constexpr (RING == 0) {
 #pragma unroll
-    for (int f = 0; f < NF; f++)
-        if (f < mine) {
-            load_step(steps[f], ids[f], step_key(f));
-            if (f + NF < mine) fetch_ids(ids[f], step_key(f + NF));
-        }
+        for (int f = 0; f < NF; f++)
+            if (f < mine) {
+                load_step(steps[f], ids[f], step_key(f));
+                if (f + NF < mine) fetch_ids(ids[f], step_key(f + NF));
+            }
+    } else {
+#pragma unroll
+        for (int f = 0; f < RING; f++)
+            if (f < mine) dma_step(ring_base + f * kSlotBytes, gid[f], step_key(f));
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+            if (RING < mine) next_id[h] = group_id(step_key(RING), h);
+    }
 #pragma unroll
     for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -705,6 +789,7 @@ __global__ __launch_bounds__(256, (D / 64) * NB <= 4 ? 2 : 1) void chunk_narrow_
 #pragma unroll
                     for (int r = 0; r < 4; r++)
                         if (16 * h + r > rel) sc[b][h][r] = -INFINITY;
+                asm volatile("" : "+v"(sc[b][0]), "+v"(sc[b][1]));      // keeps the compares inside this rarely taken branch
             }
         }
         // P against the column's current reference point; the lane's share of the sum, needed anyway, tells whether that
@@ -777,7 +862,7 @@ __global__ __launch_bounds__(256, (D / 64) * NB <= 4 ? 2 : 1) void chunk_narrow_
         }
         if (BF8 && nf) {   // rare: what the zeros stand for, added for the columns that see the key
             for (int key = t0; key <= min(t0 + STEP - 1, last_key); key++) {
-                const uint32_t *vr = reinterpret_cast<const uint32_t *>(row_at(a.v_cache, bt[entry_of(key)], key, 16 * kb));
+                const uint32_t *vr = reinterpret_cast<const uint32_t *>(row_at(a.v_cache, bt[chunk_block_of(a, key)], key, 16 * kb));
 #pragma unroll
                 for (int rb = 0; rb < RB; rb++)
 #pragma unroll
@@ -796,17 +881,38 @@ __global__ __launch_bounds__(256, (D / 64) * NB <= 4 ? 2 : 1) void chunk_narrow_
             }
         }
     };
-    for (int i = 0; i < mine; i += NF) {
+    if constexpr (RING == 0) {
+        for (int i = 0; i < mine; i += NF) {
 #pragma unroll
-        for (int f = 0; f < NF; f++) {
-            if (i + f < mine) {
-                compute_step(steps[f], step_key(i + f));
-                if (i + f + NF < mine) {
-                    load_step(steps[f], ids[f], step_key(i + f + NF));
-                    if (i + f + 2 * NF < mine) fetch_ids(ids[f], step_key(i + f + 2 * NF));
+            for (int f = 0; f < NF; f++) {
+                if (i + f < mine) {
+                    compute_step(steps[f], step_key(i + f));
+                    if (i + f + NF < mine) {
+                        load_step(steps[f], ids[f], step_key(i + f + NF));
+                        if (i + f + 2 * NF < mine) fetch_ids(ids[f], step_key(i + f + 2 * NF));
+                    }
                 }
             }
         }
+    } else {
+        uint32_t slot = ring_base;
+        for (int i = 0; i < mine; i++) {
+            // the step's loads are older than those of the RING - 1 steps behind it, kDma loads each; at the end of the
+            // range there are fewer behind it and the wave waits for all
+            if (i + RING - 1 < mine) asm volatile("s_waitcnt vmcnt(%0)" :: "n"((RING - 1) * kDma) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            ring_read<D>(slot, koff, voff, steps[0]);                // complete when it returns: the slot is free again
+            if (i + RING < mine) {
+                dma_step(slot, next_id, step_key(i + RING));
+                if (i + RING + 1 < mine) {
+                    next_id[0] = group_id(step_key(i + RING + 1), 0);
+                    next_id[1] = group_id(step_key(i + RING + 1), 1);
+                }
+            }
+            compute_step(steps[0], step_key(i));
+            slot = slot + kSlotBytes == ring_base + RING * kSlotBytes ? ring_base : slot + kSlotBytes;
+        }
+        __syncthreads();                                             // the rings become the exchange area
     }
 
     // ---- join the four waves: all partial results go to LDS, then W / NB waves finish a column block, a share of its
@@ -830,7 +936,7 @@ __global__ __launch_bounds__(256, (D / 64) * NB <= 4 ? 2 : 1) void chunk_narrow_
     constexpr int SHARES = W / NB, UNITS = RB * 4 / SHARES;
     const int b = wave / SHARES, u0 = (wave % SHARES) * UNITS;
     const int col = t.col0 + 16 * b + j;
-    if (col >= t.cols) return;
+    if (col < t.cols) {
     float m = -INFINITY, wgt[W], sum = 0.f;
 #pragma unroll
     for (int w = 0; w < W; w++) m = fmaxf(m, ml_lds[b][w][0][j]);
@@ -856,6 +962,9 @@ __global__ __launch_bounds__(256, (D / 64) * NB <= 4 ? 2 : 1) void chunk_narrow_
         else chunk_store<D, MODE>(a, it, w4, sum == 0.f ? float4_t{0.f, 0.f, 0.f, 0.f} : x * inv);
     }
     if (a.z_narrow > 1 && u0 == 0 && kb == 0) *reinterpret_cast<float2p_t *>(a.part_narrow + a.z_narrow * items * D + at * 2) = float2p_t{m, sum};
+    }
+    if (t.cols > QT) __syncthreads();                                // the next tile writes the exchange area
+    }
 }
 
 // Adds the key ranges of a column in range order.  A workgroup holds 256 / (DW * zl) items (row, head); an item's dims
@@ -977,6 +1086,9 @@ struct ChunkPlan {
     int64_t wide_bytes, narrow_bytes;   // of the workspace, per range
 };
 
+// Steps in the ring of a wave of the narrow kernel (0: the rows go through registers).
+static constexpr int ring_steps(int d, int nb) { return d == 64 ? 4 : (d == 128 ? (nb == 4 ? 4 : 2) : (d == 256 ? 2 : 0)); }
+
 static int wide_columns(int64_t d) { return d == 64 ? 256 : (d == 512 ? 64 : 128); }
 static int narrow_most_blocks(int64_t d) { return d <= 128 ? 4 : (d == 256 ? 2 : 1); }
 
@@ -997,8 +1109,7 @@ static ChunkPlan chunk_plan(int64_t n_seq, int64_t total_rows, int64_t n_q_heads
     const int most = 16 * narrow_most_blocks(d);
     const int64_t rows_most = max_q_len > 0 && max_q_len < total_rows ? max_q_len : total_rows;   // rows of the longest sequence, if the hint is right
     const int64_t cols = rows_most * group;
-    const int64_t slots_each = n_seq > 0 ? (total_rows * group / 16 + n_seq) / n_seq : 1;
-    if (cols <= most && slots_each < 4096) {                 // all sequences are short (or the hint is wrong: more tiles each)
+    if (cols <= most) {                 // all sequences are short (or the hint is wrong: more tiles each)
         p.narrow = true;
         p.wide = false;
         p.col_split = kAnyColumns;
@@ -1044,38 +1155,37 @@ static int launch_chunk_wide(const ChunkArgs &a, bool fill, hipStream_t s) {
     return check_launch(me);
 }
 
-template <int D, int MODE, int NB, bool POW2>
+template <int D, int MODE, int NB, int RING>
 static int launch_chunk_narrow(const ChunkArgs &a, bool fill, hipStream_t s) {
-    constexpr size_t lds = (size_t)NB * 4 * (D / 64) * 4 * 64 * 16;
+    constexpr size_t join = (size_t)NB * 4 * (D / 64) * 4 * 64 * 16, rings = (size_t)4 * RING * 64 * D, lds = join > rings ? join : rings;
     const char *me = "feather_paged_chunk_attn_fp8";
-    const int64_t slots = a.col_split < kAnyColumns ? a.n_seq : chunk_slots(a.total_rows, a.n_seq, a.group, 16 * NB);
-    const int64_t each = a.n_seq > 0 ? (slots + a.n_seq - 1) / a.n_seq : 1, pairs = a.n_seq > 0 ? (int64_t)a.n_seq * a.n_kv_heads : kChunkFillGroups;
-    FEATHER_CHECK(pairs < (1ll << 31) && each < 65536 && pairs * each * a.z_narrow < (1ll << 31), FEATHER_ESHAPE, "%s: grid too large", me);
-    auto kern = chunk_narrow_kernel<D, MODE, NB, POW2>;
+    const int64_t pairs = a.n_seq > 0 ? (int64_t)a.n_seq * a.n_kv_heads : kChunkFillGroups;
+    FEATHER_CHECK(pairs * a.z_narrow < (1ll << 31), FEATHER_ESHAPE, "%s: grid too large", me);
+    auto kern = chunk_narrow_kernel<D, MODE, NB, RING>;
     static unsigned long long lds_raised = 0;
     hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(kern), lds + 4096, lds_raised);
     FEATHER_CHECK(e == hipSuccess, FEATHER_ELAUNCH, "%s: cannot raise LDS limit: %s", me, hipGetErrorString(e));
-    hipLaunchKernelGGL(kern, dim3((unsigned)pairs, (unsigned)a.z_narrow, (unsigned)each), dim3(256), lds, s, a, (int)slots, fill ? 1 : 0);
+    hipLaunchKernelGGL(kern, dim3((unsigned)pairs, (unsigned)a.z_narrow), dim3(256), lds, s, a, fill ? 1 : 0);
     return check_launch(me);
 }
 
-template <int D, int MODE, bool POW2>
+template <int D, int MODE, bool PAGE16>
 static int launch_chunk(const ChunkArgs &a, const ChunkPlan &p, hipStream_t s) {
     constexpr int QB = D == 64 ? 4 : (D == 128 ? 2 : 1), BN = D == 512 ? 32 : 64, OCC = D <= 128 ? 2 : 1, WAVES = D == 256 ? 8 : 4;
     const bool merge = a.z_wide > 1 || a.z_narrow > 1;
     bool fill = a.fill && !merge;                            // rows outside every sequence: the merge's work, or the first kernel's
     int rc = FEATHER_OK;
     if (p.wide) {
-        rc = a.z_wide > 1 ? launch_chunk_wide<D, MODE, QB, BN, OCC, WAVES, POW2, true>(a, fill, s)
-                          : launch_chunk_wide<D, MODE, QB, BN, OCC, WAVES, POW2, false>(a, fill, s);
+        rc = a.z_wide > 1 ? launch_chunk_wide<D, MODE, QB, BN, OCC, WAVES, PAGE16, true>(a, fill, s)
+                          : launch_chunk_wide<D, MODE, QB, BN, OCC, WAVES, PAGE16, false>(a, fill, s);
         fill = false;
     }
     if (rc == FEATHER_OK && p.narrow) {
-        if (p.nb == 1) rc = launch_chunk_narrow<D, MODE, 1, POW2>(a, fill, s);
+        if (p.nb == 1) rc = launch_chunk_narrow<D, MODE, 1, PAGE16 ? ring_steps(D, 1) : 0>(a, fill, s);
         if constexpr (D <= 256)
-            if (p.nb == 2) rc = launch_chunk_narrow<D, MODE, 2, POW2>(a, fill, s);
+            if (p.nb == 2) rc = launch_chunk_narrow<D, MODE, 2, PAGE16 ? ring_steps(D, 2) : 0>(a, fill, s);
         if constexpr (D <= 128)
-            if (p.nb == 4) rc = launch_chunk_narrow<D, MODE, 4, POW2>(a, fill, s);
+            if (p.nb == 4) rc = launch_chunk_narrow<D, MODE, 4, PAGE16 ? ring_steps(D, 4) : 0>(a, fill, s);
     }
     if (rc != FEATHER_OK || !merge) return rc;
     constexpr int DW = D / 4;
@@ -1087,13 +1197,13 @@ static int launch_chunk(const ChunkArgs &a, const ChunkPlan &p, hipStream_t s) {
     return check_launch("feather_paged_chunk_attn_fp8 (merge of the key ranges)");
 }
 
-template <int MODE, bool POW2>
+template <int MODE, bool PAGE16>
 static int dispatch_chunk(const ChunkArgs &a, const ChunkPlan &p, int64_t d, hipStream_t s) {
     switch (d) {
-        case 64: return launch_chunk<64, MODE, POW2>(a, p, s);
-        case 128: return launch_chunk<128, MODE, POW2>(a, p, s);
-        case 256: return launch_chunk<256, MODE, POW2>(a, p, s);
-        default: return launch_chunk<512, MODE, POW2>(a, p, s);
+        case 64: return launch_chunk<64, MODE, PAGE16>(a, p, s);
+        case 128: return launch_chunk<128, MODE, PAGE16>(a, p, s);
+        case 256: return launch_chunk<256, MODE, PAGE16>(a, p, s);
+        default: return launch_chunk<512, MODE, PAGE16>(a, p, s);
     }
 }
 
@@ -1170,7 +1280,7 @@ extern "C" int feather_paged_chunk_attn_fp8(const void *q, const void *k_cache, 
     a.part_narrow = reinterpret_cast<float *>(static_cast<char *>(scratch) + chunk_wide_scratch(p)); a.col_split = p.col_split;
     a.scale_log2e = scale * 1.4426950408889634f;
     hipStream_t s = (hipStream_t)stream;
-    const bool al = block_size % 4 == 0 && (block_size & (block_size - 1)) == 0;
+    const bool al = block_size % 16 == 0;
     if (mode == FEATHER_E5M2) return al ? dispatch_chunk<FEATHER_E5M2, true>(a, p, d, s) : dispatch_chunk<FEATHER_E5M2, false>(a, p, d, s);
     return al ? dispatch_chunk<FEATHER_E4M3, true>(a, p, d, s) : dispatch_chunk<FEATHER_E4M3, false>(a, p, d, s);
 }
