@@ -208,15 +208,17 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn_kernel(ChunkArgs a
         chunk_fill_outside<D>(a, bid - work, gridDim.x - work, kThreads);
         return;
     }
-    if (work % 8 == 0) bid = (bid % 8) * (work / 8) + bid / 8;   // an XCD (own L2) works through neighbouring tiles of one KV head
+    // Launch order goes round the XCDs (own L2 each): with the KV head fastest an XCD keeps to few heads, and with the tiles
+    // slowest the longest tiles of all heads start first on all of them.
+    const int kvh = bid % a.n_kv_heads;
+    bid /= a.n_kv_heads;
     int zr = 0;
     if constexpr (ZS) {
         zr = bid % a.z_wide;
         bid /= a.z_wide;
     }
-    const int kvh = bid / n_slots;
     ChunkTile t;
-    if (!chunk_find_tile(a, bid % n_slots, QT, t)) return;
+    if (!chunk_find_tile(a, bid, QT, t)) return;
     if (t.cols <= a.col_split) return;                 // a short run of rows: the other kernel's work
 
     int key_begin = 0, key_end = t.keys;
@@ -375,7 +377,7 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn_kernel(ChunkArgs a
             fetch_ids(key_begin + 2 * BN);
         }
     }
-    if (BF8 && a.causal) nf = __syncthreads_or(nf);
+    if (BF8 && key_begin < key_end && on_diag(key_begin)) nf = __syncthreads_or(nf);
     else __syncthreads();
     int cur = 0;
     for (int key0 = key_begin; key0 < key_end; key0 += BN, cur ^= 1) {
@@ -485,8 +487,13 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn_kernel(ChunkArgs a
                 }
             }
         }
-        if (BF8 && a.causal) nf = __syncthreads_or(nf_next);
-        else __syncthreads();
+        // only a tile on the diagonal can have something to report (the vote costs more than the barrier)
+        if (BF8 && key0 + BN < key_end && on_diag(key0 + BN)) {
+            nf = __syncthreads_or(nf_next);
+        } else {
+            nf = 0;
+            __syncthreads();
+        }
     }
 
     if (!wave_has) return;
@@ -504,6 +511,369 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn_kernel(ChunkArgs a
 #pragma unroll
             for (int d = 0; d < DB; d++) chunk_store<D, MODE>(a, item[b], 4 * d + kb, l == 0.f ? float4_t{0.f, 0.f, 0.f, 0.f} : o[b][d] * inv);
         }
+    }
+}
+
+// ---- d = 64: tiles through LDS on the 32x32 matrix instructions ---------------------------------------------------------
+// The split and the numerics of chunk_attn_kernel, and the instruction mix of the prefill kernel's d = 64 form: vector
+// issue bounds this head dim, and an instruction of 32x32 holds it half as long per product as two of 16x16 --
+//     S^T[32 keys, 32 cols] = v_mfma_f32_32x32x64_f8f6f4 (E5M2 bytes as they are: the whole head dim) or four of
+//                             v_mfma_f32_32x32x16_f16 (E4M3, decoded);   O^T[32 dims, 32 cols] += v_mfma_f32_32x32x16_f16
+// A wave owns 32 * CB columns.  Lane l: n = l % 32 the column, h = l / 32; accumulator register r is row
+// 8 (r / 4) + 4 h + r % 4.  Registers 8 s .. 8 s + 7 of the scores are the k-slots of the second product's step s if V^T
+// holds the keys of every group of 16 in the order 0 1 2 3 8 9 10 11 | 4 5 6 7 12 13 14 15.
+// PAGE16 (block_size % 16 == 0): the 16 keys that a wave stages share a block, whose address is then scalar.
+typedef int int8p_t __attribute__((ext_vector_type(8)));
+
+template <int MODE, int CB, int WAVES, int OCC, bool PAGE16, bool ZS>
+__global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn64_kernel(ChunkArgs a, int n_slots) {
+    constexpr int D = 64, DW = 16, BN = 64;
+    constexpr bool BF8 = MODE == FEATHER_E5M2;
+    constexpr int KP = (BF8 ? D : 2 * D) + 16;   // K row pitch in LDS, bytes
+    constexpr int VS = BN;                       // fp16 per V^T row
+    constexpr int kThreads = 64 * WAVES, QT = 32 * CB * WAVES;
+    constexpr int kBufBytes = BN * KP + D * VS * 2;
+    static_assert(kThreads >= 256, "256 threads stage a tile");
+
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    auto swz = [](int row) { return ((row >> 1) & 7) ^ ((row >> 4) & 1); };   // 16-byte chunk c of V^T row r lives at chunk c ^ swz(r)
+
+    const int work = n_slots * a.n_kv_heads * (ZS ? a.z_wide : 1);
+    int bid = blockIdx.x;
+    if (bid >= work) {
+        chunk_fill_outside<D>(a, bid - work, gridDim.x - work, kThreads);
+        return;
+    }
+    // Launch order goes round the XCDs (own L2 each): with the KV head fastest an XCD keeps to few heads, and with the tiles
+    // slowest the longest tiles of all heads start first on all of them.
+    const int kvh = bid % a.n_kv_heads;
+    bid /= a.n_kv_heads;
+    int zr = 0;
+    if constexpr (ZS) {
+        zr = bid % a.z_wide;
+        bid /= a.z_wide;
+    }
+    ChunkTile t;
+    if (!chunk_find_tile(a, bid, QT, t)) return;
+    if (t.cols <= a.col_split) return;                 // a short run of rows: the other kernel's work
+    int key_begin = 0, key_end = t.keys;
+    if constexpr (ZS) {
+        const int per = chunk_range_keys(t.keys, a.z_wide, BN, kChunkMinKeys);
+        key_begin = zr * per;
+        key_end = min(t.keys, key_begin + per);
+        if (key_begin >= key_end) return;              // the merge knows which ranges exist
+    }
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
+    const int n = lane & 31, h = lane >> 5;
+    const int qc0 = t.col0 + wave * (32 * CB);
+    const int32_t *bt = a.block_tables + (int64_t)t.seq * a.max_blocks;
+    const uint32_t block_bytes = (uint32_t)(a.n_kv_heads * a.block_size) * D;
+    const int64_t head_bytes = (int64_t)kvh * a.block_size * D;
+    auto slot_of = [&](int pos) { return (uint32_t)pos - chunk_block_of(a, pos) * (uint32_t)a.block_size; };
+    auto row_at = [&](const uint32_t *cache, int id, int pos) {
+        return reinterpret_cast<const char *>(cache) + ((uint64_t)min((uint32_t)id, a.max_blk) * block_bytes + (uint64_t)head_bytes + slot_of(pos) * D);
+    };
+
+    int64_t item[CB];
+    int last[CB];
+#pragma unroll
+    for (int b = 0; b < CB; b++) {
+        const int c = min(qc0 + 32 * b + n, t.cols - 1), r = chunk_row_of(a, c);
+        item[b] = (int64_t)(t.row0 + r) * a.n_q_heads + kvh * a.group + (c - r * a.group);
+        last[b] = a.causal ? t.p0 + r : t.ctx - 1;
+    }
+    const int wave_first = a.causal ? t.p0 + chunk_row_of(a, min(qc0, t.cols - 1)) : t.ctx - 1;
+    const int wave_last = a.causal ? t.p0 + chunk_row_of(a, min(qc0 + 32 * CB - 1, t.cols - 1)) : t.ctx - 1;
+    const int tile_first = a.causal ? t.p0 + chunk_row_of(a, t.col0) : t.ctx - 1;
+    const bool wave_has = qc0 < t.cols;
+
+    int8p_t qf[BF8 ? CB : 1];
+    half8_t qh16[BF8 ? 1 : CB][BF8 ? 1 : 4];
+#pragma unroll
+    for (int b = 0; b < CB; b++) {
+        if constexpr (BF8) {
+            const u32x2 *src = reinterpret_cast<const u32x2 *>(a.q + item[b] * DW + 8 * h);   // q need not be aligned to 16 bytes
+            const u32x2 w0 = src[0], w1 = src[1], w2 = src[2], w3 = src[3];
+            qf[b] = int8p_t{(int)w0.x, (int)w0.y, (int)w1.x, (int)w1.y, (int)w2.x, (int)w2.y, (int)w3.x, (int)w3.y};
+        } else {
+#pragma unroll
+            for (int st = 0; st < 4; st++) {
+                const u32x2 w = *reinterpret_cast<const u32x2 *>(a.q + item[b] * DW + 4 * st + 2 * h);
+                qh16[b][st] = chunk_dec8<MODE>(w.x, w.y);
+            }
+        }
+    }
+
+    float16_t o[CB][2];                          // [32-dim block]
+    float m_run[CB], mc_run[CB], l_run[CB];      // reference point (raw, and times scale * log2 e), the lane's share of the sum
+#pragma unroll
+    for (int b = 0; b < CB; b++) {
+        m_run[b] = mc_run[b] = -INFINITY;
+        l_run[b] = 0.f;
+#pragma unroll
+        for (int d = 0; d < 2; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[b][d][r] = 0.f;
+    }
+
+    // ---- staging: 256 threads carry V (4 keys x 4 dims each), 256 threads K (16 bytes of one key each): the same ones in a
+    // four-wave workgroup, waves 0-3 and 4-7 in an eight-wave one.  A wave's keys are 16 neighbours in both.
+    constexpr bool kSplit = kThreads >= 512;
+    const bool stages_v = tid < 256, stages_k = kSplit ? tid >= 256 : tid < 256;
+    const int kt = kSplit ? tid - 256 : tid;     // index among the K stagers
+    const int key16 = 16 * (wave & 3);           // the wave's first key inside a tile
+    const __attribute__((address_space(4))) int32_t *bt_const = (const __attribute__((address_space(4))) int32_t *)bt;   // read only while the kernel runs: scalar loads
+    int id_k = 0, id_v[4] = {0, 0, 0, 0};        // PAGE16: id_k only, wave-uniform
+    auto fetch_ids = [&](int key0) {
+        if constexpr (PAGE16) {
+            id_k = bt_const[chunk_block_of(a, min(key0 + key16, (key_end - 1) & ~15))];
+        } else {
+            if (stages_k) id_k = bt[chunk_block_of(a, min(key0 + kt / 4, key_end - 1))];
+            if (stages_v)
+#pragma unroll
+                for (int r = 0; r < 4; r++) id_v[r] = bt[chunk_block_of(a, min(key0 + 4 * (tid / DW) + r, key_end - 1))];
+        }
+    };
+    u32x4 kreg;
+    uint32_t vreg[4];
+    auto prefetch = [&](int key0) {              // keys past the end: another key's row (masked; its V is zeroed by `stage`)
+        if constexpr (PAGE16) {
+            const int pos = min(key0 + key16, (key_end - 1) & ~15);
+            if (stages_k) kreg = *reinterpret_cast<const u32x4 *>(row_at(a.k_cache, id_k, pos) + (uint32_t)((kt / 4 % 16) * D + 16 * (kt % 4)));
+            if (stages_v) {
+                const char *vr = row_at(a.v_cache, id_k, pos) + (uint32_t)((tid / DW % 4) * 4 * D + 4 * (tid % DW));
+#pragma unroll
+                for (int r = 0; r < 4; r++) vreg[r] = *reinterpret_cast<const uint32_t *>(vr + r * D);
+            }
+        } else {
+            if (stages_k) kreg = *reinterpret_cast<const u32x4 *>(row_at(a.k_cache, id_k, min(key0 + kt / 4, key_end - 1)) + 16 * (kt % 4));
+            if (stages_v)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    vreg[r] = *reinterpret_cast<const uint32_t *>(row_at(a.v_cache, id_v[r], min(key0 + 4 * (tid / DW) + r, key_end - 1)) + 4 * (tid % DW));
+        }
+    };
+    auto on_diag = [&](int key0) { return min(key0 + BN, key_end) - 1 > tile_first; };   // some column does not see some key of the tile
+    // decodes the fetched tile into buffer `buf`; E5M2: codes of inf and NaN in V are staged as zero where a column does not
+    // see some key of the tile (P = 0 there, and 0 * inf is NaN), and reported
+    auto stage = [&](int buf, int key0) -> int {
+        int nf = 0;
+        unsigned char *k_lds = smem + buf * kBufBytes;
+        _Float16 *vt_lds = reinterpret_cast<_Float16 *>(k_lds + BN * KP);
+        if (stages_k) {
+            const int key = kt / 4, c16 = kt % 4;
+            if constexpr (BF8) {
+                *reinterpret_cast<u32x4 *>(k_lds + key * KP + 16 * c16) = kreg;
+            } else {
+                half8_t *kd = reinterpret_cast<half8_t *>(k_lds + key * KP + 32 * c16);
+                kd[0] = chunk_dec8<MODE>(kreg.x, kreg.y);
+                kd[1] = chunk_dec8<MODE>(kreg.z, kreg.w);
+            }
+        }
+        if (stages_v) {
+            const int ddw = tid % DW, kg = tid / DW;
+            const int q4 = kg & 3, pos = 16 * (kg >> 2) + 8 * (q4 & 1) + 4 * (q4 >> 1);
+            const bool whole = key0 + BN <= key_end;
+            if (!whole)
+#pragma unroll
+                for (int r = 0; r < 4; r++) vreg[r] = key0 + 4 * kg + r < key_end ? vreg[r] : 0u;
+            uint32_t lo2[4], hi2[4];             // halfs (key 0, key 1) and (key 2, key 3) of dim 4 ddw + c
+            if constexpr (BF8) {
+                if (on_diag(key0)) {
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const uint32_t m = chunk_nonfinite(vreg[r]);
+                        vreg[r] &= ~m;
+                        nf |= m != 0;
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const uint32_t sel = 0x000c000cu | ((uint32_t)c << 8) | ((uint32_t)(4 + c) << 24);
+                    lo2[c] = perm(vreg[1], vreg[0], sel);
+                    hi2[c] = perm(vreg[3], vreg[2], sel);
+                }
+            } else {
+                uint32_t p01[4], p23[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) dec_word<MODE>(vreg[r], p01[r], p23[r]);
+                lo2[0] = perm(p01[1], p01[0], 0x05040100u); hi2[0] = perm(p01[3], p01[2], 0x05040100u);
+                lo2[1] = perm(p01[1], p01[0], 0x07060302u); hi2[1] = perm(p01[3], p01[2], 0x07060302u);
+                lo2[2] = perm(p23[1], p23[0], 0x05040100u); hi2[2] = perm(p23[3], p23[2], 0x05040100u);
+                lo2[3] = perm(p23[1], p23[0], 0x07060302u); hi2[3] = perm(p23[3], p23[2], 0x07060302u);
+            }
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const int row = 4 * ddw + c;
+                *reinterpret_cast<u32x2 *>(vt_lds + row * VS + (((pos >> 3) ^ swz(row)) << 3) + (pos & 4)) = u32x2{lo2[c], hi2[c]};
+            }
+        }
+        return nf;
+    };
+
+    int nf = 0;
+    if (key_begin < key_end) {
+        fetch_ids(key_begin);
+        prefetch(key_begin);
+        fetch_ids(key_begin + BN);
+        nf = stage(0, key_begin);
+        if (key_begin + BN < key_end) {
+            prefetch(key_begin + BN);
+            fetch_ids(key_begin + 2 * BN);
+        }
+    }
+    if (BF8 && key_begin < key_end && on_diag(key_begin)) nf = __syncthreads_or(nf);
+    else __syncthreads();
+    // one tile; the buffer index is a compile-time constant, so LDS addresses are loop-invariant registers plus immediates
+    auto tile_body = [&](const int key0, auto cur_c) {
+        constexpr int cur = decltype(cur_c)::value;
+        const unsigned char *k_lds = smem + cur * kBufBytes;
+        const _Float16 *vt_lds = reinterpret_cast<const _Float16 *>(k_lds + BN * KP);
+        int nf_next = 0;
+        if (key0 + BN < key_end) {
+            nf_next = stage(cur ^ 1, key0 + BN);
+            if (key0 + 2 * BN < key_end) {
+                prefetch(key0 + 2 * BN);
+                fetch_ids(key0 + 3 * BN);
+            }
+        }
+        const bool masked = key0 + BN - 1 > wave_first;           // wave-uniform: some column does not see some key
+        if (wave_has && key0 <= wave_last) {
+            half8_t vf[4][2];   // [16-key step][32-dim block]
+#pragma unroll
+            for (int g = 0; g < 4; g++)
+#pragma unroll
+                for (int d = 0; d < 2; d++) {
+                    const int row = 32 * d + n;
+                    vf[g][d] = *reinterpret_cast<const half8_t *>(vt_lds + row * VS + (((2 * g + h) ^ swz(row)) << 3));
+                }
+            float16_t sc[CB][2];
+            const float16_t zero16 = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                if constexpr (BF8) {
+                    const u32x4 *src = reinterpret_cast<const u32x4 *>(k_lds + (32 * c + n) * KP + 32 * h);
+                    const u32x4 w0 = src[0], w1 = src[1];
+                    const int8p_t kf = {(int)w0.x, (int)w0.y, (int)w0.z, (int)w0.w, (int)w1.x, (int)w1.y, (int)w1.z, (int)w1.w};
+#pragma unroll
+                    for (int b = 0; b < CB; b++)   // both operands in the BF8 (E5M2) format, no block scales
+                        sc[b][c] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf, qf[b], zero16, 1, 1, 0, 0, 0, 0);
+                } else {
+                    half8_t k16[4];
+#pragma unroll
+                    for (int st = 0; st < 4; st++) k16[st] = *reinterpret_cast<const half8_t *>(k_lds + (32 * c + n) * KP + 32 * st + 16 * h);
+#pragma unroll
+                    for (int b = 0; b < CB; b++)
+#pragma unroll
+                        for (int st = 0; st < 4; st++)
+                            sc[b][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k16[st], qh16[b][st], st == 0 ? zero16 : sc[b][c], 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < CB; b++) {
+                if (masked) {
+                    int rel = last[b] - key0 - 4 * h;             // key 32 c + 8 (r / 4) + 4 h + r % 4 is hidden if 32 c + 8 (r / 4) + r % 4 > rel
+                    asm volatile("" : "+v"(rel));                 // keeps the 32 compares inside this rarely taken branch
+#pragma unroll
+                    for (int c = 0; c < 2; c++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++)
+                            if (32 * c + 8 * (r >> 2) + (r & 3) > rel) sc[b][c][r] = -INFINITY;
+                }
+                // P against the column's current reference point; the lane's share of the sum tells whether that was safe
+                // (see kGuard); if not, the reference is raised to the true maximum and P computed again
+                half8_t pb[4];
+                auto exp_block = [&](const float mc) {
+                    float sum = 0.f;
+#pragma unroll
+                    for (int g = 0; g < 4; g++) {
+                        uint32_t pw[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][g >> 1][8 * (g & 1) + 2 * i], a.scale_log2e, -mc));
+                            const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][g >> 1][8 * (g & 1) + 2 * i + 1], a.scale_log2e, -mc));
+                            pw[i] = as_u32(__builtin_convertvector(float2p_t{e0, e1}, half2_t));
+                            sum = dot2(pw[i], 0x3c003c00u, sum);  // the sum takes the rounded values that multiply V
+                        }
+                        pb[g] = __builtin_bit_cast(half8_t, u32x4{pw[0], pw[1], pw[2], pw[3]});
+                    }
+                    return sum;
+                };
+                float sum = exp_block(mc_run[b]);
+                if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(sum < kGuard)) != 0, 0)) {
+                    float mx = max3_raw(sc[b][0][0], sc[b][0][1], sc[b][0][2]);
+                    mx = max_raw(mx, sc[b][0][3]);
+#pragma unroll
+                    for (int i = 2; i < 16; i++) mx = max3_raw(mx, sc[b][i >> 3][(2 * i) & 15], sc[b][i >> 3][(2 * i + 1) & 15]);
+                    mx = max_xor32(mx);                           // the two lanes of a column
+                    const float m_old = m_run[b], m_new = max_raw(m_old, mx);
+                    // a column that has seen no key keeps the reference -inf: its scores are -inf here, its P zero
+                    const float alpha = m_old == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_old - m_new) * a.scale_log2e);
+                    m_run[b] = m_new;
+                    mc_run[b] = m_new * a.scale_log2e;
+                    l_run[b] *= alpha;
+#pragma unroll
+                    for (int d = 0; d < 2; d++) o[b][d] *= alpha;
+                    sum = exp_block(m_new == -INFINITY ? 0.f : mc_run[b]);
+                }
+                l_run[b] += sum;
+#pragma unroll
+                for (int g = 0; g < 4; g++)
+#pragma unroll
+                    for (int d = 0; d < 2; d++) o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[g][d], pb[g], o[b][d], 0, 0, 0);
+            }
+            if (BF8 && nf) {   // rare: what the staged zeros stand for, added for the columns that see the key
+                for (int key = key0; key < min(key0 + BN, key_end); key++) {
+                    const uint32_t *vr = reinterpret_cast<const uint32_t *>(row_at(a.v_cache, bt[chunk_block_of(a, key)], key)) + h;
+#pragma unroll
+                    for (int d = 0; d < 2; d++)
+#pragma unroll
+                        for (int g = 0; g < 4; g++) {             // dims 32 d + 8 g + 4 h + {0..3}
+                            const uint32_t w = vr[8 * d + 2 * g], m = chunk_nonfinite(w);
+                            if (m != 0)
+#pragma unroll
+                                for (int r = 0; r < 4; r++)
+                                    if ((m >> (8 * r)) & 1u) {
+                                        const float x = (float)__builtin_bit_cast(_Float16, (uint16_t)((w >> (8 * r)) << 8));
+#pragma unroll
+                                        for (int b = 0; b < CB; b++)
+                                            if (key <= last[b]) o[b][d][4 * g + r] += x;
+                                    }
+                        }
+                }
+            }
+        }
+        // only a tile on the diagonal can have something to report (the vote costs more than the barrier)
+        if (BF8 && key0 + BN < key_end && on_diag(key0 + BN)) {
+            nf = __syncthreads_or(nf_next);
+        } else {
+            nf = 0;
+            __syncthreads();
+        }
+    };
+    for (int key0 = key_begin; key0 < key_end; key0 += 2 * BN) {
+        tile_body(key0, std::integral_constant<int, 0>{});
+        if (key0 + BN < key_end) tile_body(key0 + BN, std::integral_constant<int, 1>{});
+    }
+
+    if (!wave_has) return;
+#pragma unroll
+    for (int b = 0; b < CB; b++) {
+        const float l = l_run[b] + as_float((uint32_t)__builtin_amdgcn_ds_bpermute(4 * (lane ^ 32), (int)as_u32(l_run[b])));
+        if (qc0 + 32 * b + n >= t.cols) continue;
+        const int64_t items = (int64_t)a.total_rows * a.n_q_heads, at = zr * items + item[b];
+        const float inv = l == 0.f ? 0.f : 1.0f / l;              // no visible key: a zero result
+#pragma unroll
+        for (int d = 0; d < 2; d++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const float4_t x = {o[b][d][4 * g], o[b][d][4 * g + 1], o[b][d][4 * g + 2], o[b][d][4 * g + 3]};
+                if constexpr (ZS) *reinterpret_cast<float4_t *>(a.part + at * D + 32 * d + 8 * g + 4 * h) = x;
+                else chunk_store<D, MODE>(a, item[b], 8 * d + 2 * g + h, l == 0.f ? float4_t{0.f, 0.f, 0.f, 0.f} : x * inv);
+            }
+        if constexpr (ZS)
+            if (h == 0) *reinterpret_cast<float2p_t *>(a.part + a.z_wide * items * D + at * 2) = float2p_t{m_run[b], l};
     }
 }
 
@@ -1089,6 +1459,8 @@ struct ChunkPlan {
 // Steps in the ring of a wave of the narrow kernel (0: the rows go through registers).
 static constexpr int ring_steps(int d, int nb) { return d == 64 ? 4 : (d == 128 ? (nb == 4 ? 4 : 2) : (d == 256 ? 2 : 0)); }
 
+constexpr int kWide64Blocks = 2;   // 32-column blocks of a wave of the d = 64 kernel (256 columns per workgroup)
+
 static int wide_columns(int64_t d) { return d == 64 ? 256 : (d == 512 ? 64 : 128); }
 static int narrow_most_blocks(int64_t d) { return d <= 128 ? 4 : (d == 256 ? 2 : 1); }
 
@@ -1122,7 +1494,7 @@ static ChunkPlan chunk_plan(int64_t n_seq, int64_t total_rows, int64_t n_q_heads
     }
     p.narrow_rows = p.wide && p.narrow ? (int)(p.col_split / group) : 0;
     const int64_t each = n_seq > 0 ? (total_rows + n_seq - 1) / n_seq * group : 1;   // columns of a sequence of average length
-    p.z_wide = p.wide ? ranges_for((total_rows * group / wide_columns(d) + 1) * n_kv_heads, 512, max_ctx, kChunkMinKeys) : 1;
+    p.z_wide = p.wide ? ranges_for(n_seq * ((each + wide_columns(d) - 1) / wide_columns(d)) * n_kv_heads, 512, max_ctx, kChunkMinKeys) : 1;
     // the chip holds 256 workgroups of a kernel that fills a CU's registers, two or three times as many of a smaller one
     const int weight = (int)(d / 64) * p.nb;
     const int64_t groups = 256 * (weight <= 2 ? 3 : (weight <= 4 ? 2 : 1));
@@ -1138,20 +1510,25 @@ static ChunkPlan chunk_plan(int64_t n_seq, int64_t total_rows, int64_t n_q_heads
 static int64_t chunk_wide_scratch(const ChunkPlan &p) { return p.z_wide > 1 ? (p.z_wide * p.wide_bytes + 15) / 16 * 16 : 0; }
 static int64_t chunk_narrow_scratch(const ChunkPlan &p) { return p.z_narrow > 1 ? p.z_narrow * p.narrow_bytes + 16 : 0; }
 
-template <int D, int MODE, int QB, int BN, int OCC, int WAVES, bool ALIGN4, bool ZS>
+template <int D, int MODE, bool PAGE16, bool ZS>
 static int launch_chunk_wide(const ChunkArgs &a, bool fill, hipStream_t s) {
-    constexpr int QT = 16 * QB * WAVES;
+    constexpr int QB = D == 128 ? 2 : 1, BN = D == 512 ? 32 : 64, OCC = D <= 128 ? 2 : 1, WAVES = D == 256 ? 8 : 4;
+    constexpr int QT = D == 64 ? 256 : 16 * QB * WAVES;
     constexpr int KS = MODE == FEATHER_E5M2 ? (D + 16) / 2 : D + 8;
     constexpr size_t lds = (size_t)(BN * KS + D * BN) * 2 * 2;
     const char *me = "feather_paged_chunk_attn_fp8";
     const int64_t slots = chunk_slots(a.total_rows, a.n_seq, a.group, QT);
     const int64_t blocks = slots * a.n_kv_heads * a.z_wide;
     FEATHER_CHECK(blocks + kChunkFillGroups < (1ll << 31), FEATHER_ESHAPE, "%s: grid too large", me);
-    auto kern = chunk_attn_kernel<D, MODE, QB, BN, OCC, WAVES, ALIGN4, ZS>;
+    auto kern = [] {
+        if constexpr (D == 64) return chunk_attn64_kernel<MODE, kWide64Blocks, 256 / (32 * kWide64Blocks), 2, PAGE16, ZS>;
+        else return chunk_attn_kernel<D, MODE, QB, BN, OCC, WAVES, PAGE16, ZS>;
+    }();
+    constexpr int threads = D == 64 ? 64 * (256 / (32 * kWide64Blocks)) : 64 * WAVES;
     static unsigned long long lds_raised = 0;
     hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(kern), lds, lds_raised);
     FEATHER_CHECK(e == hipSuccess, FEATHER_ELAUNCH, "%s: cannot raise LDS limit: %s", me, hipGetErrorString(e));
-    hipLaunchKernelGGL(kern, dim3((unsigned)(blocks + (fill ? kChunkFillGroups : 0))), dim3(64 * WAVES), lds, s, a, (int)slots);
+    hipLaunchKernelGGL(kern, dim3((unsigned)(blocks + (fill ? kChunkFillGroups : 0))), dim3(threads), lds, s, a, (int)slots);
     return check_launch(me);
 }
 
@@ -1171,13 +1548,12 @@ static int launch_chunk_narrow(const ChunkArgs &a, bool fill, hipStream_t s) {
 
 template <int D, int MODE, bool PAGE16>
 static int launch_chunk(const ChunkArgs &a, const ChunkPlan &p, hipStream_t s) {
-    constexpr int QB = D == 64 ? 4 : (D == 128 ? 2 : 1), BN = D == 512 ? 32 : 64, OCC = D <= 128 ? 2 : 1, WAVES = D == 256 ? 8 : 4;
     const bool merge = a.z_wide > 1 || a.z_narrow > 1;
     bool fill = a.fill && !merge;                            // rows outside every sequence: the merge's work, or the first kernel's
     int rc = FEATHER_OK;
     if (p.wide) {
-        rc = a.z_wide > 1 ? launch_chunk_wide<D, MODE, QB, BN, OCC, WAVES, PAGE16, true>(a, fill, s)
-                          : launch_chunk_wide<D, MODE, QB, BN, OCC, WAVES, PAGE16, false>(a, fill, s);
+        rc = a.z_wide > 1 ? launch_chunk_wide<D, MODE, PAGE16, true>(a, fill, s)
+                          : launch_chunk_wide<D, MODE, PAGE16, false>(a, fill, s);
         fill = false;
     }
     if (rc == FEATHER_OK && p.narrow) {
@@ -1193,7 +1569,7 @@ static int launch_chunk(const ChunkArgs &a, const ChunkPlan &p, hipStream_t s) {
     while (!p.wide && zl * 4 < a.z_narrow && zl * DW < 256) zl *= 2;
     const int64_t per_group = 256 / (DW * zl), items = (int64_t)a.total_rows * a.n_q_heads;
     hipLaunchKernelGGL((chunk_merge_kernel<D, MODE>), dim3((unsigned)((items + per_group - 1) / per_group)), dim3(256), 0, s, a,
-                       16 * QB * WAVES, BN, 16 * p.nb, zl);
+                       wide_columns(D), D == 512 ? 32 : 64, 16 * p.nb, zl);
     return check_launch("feather_paged_chunk_attn_fp8 (merge of the key ranges)");
 }
 
