@@ -65,6 +65,8 @@ struct ForkArgs {
     int32_t *free_count;    // [chunks] free blocks of a chunk
     int32_t *free_ids;      // [n_blocks] their ids, chunk by chunk
     int n_seq, max_blocks, block_size, n_blocks, chunk, chunks;
+    uint32_t row_mul;       // i / max_blocks = umulhi(2 i, row_mul) >> row_shift for 0 <= i < 2^31
+    int row_shift;
 };
 
 constexpr int kFreshTail = -2, kFreshRoom = -3;   // entries of a new row that still wait for a block
@@ -77,24 +79,33 @@ __global__ __launch_bounds__(kPgChunkThreads) void fork_plan_kernel(ForkArgs a) 
     __shared__ int red[kPgChunkThreads / kWave];
     const int tid = threadIdx.x, cap = a.max_blocks * a.block_size;
     if ((int)blockIdx.x < a.chunks) {
-        int *count = pg_lds, *children = pg_lds + a.chunk;
+        int *count = pg_lds, *children = pg_lds + a.chunk, *whole = children + a.n_seq;
         const int b0 = blockIdx.x * a.chunk, n = min(a.chunk, a.n_blocks - b0);
         for (int i = tid; i < n; i += kPgChunkThreads) count[i] = a.ref[b0 + i];
-        for (int i = tid; i < a.n_seq; i += kPgChunkThreads) children[i] = 0;
+        for (int i = tid; i < a.n_seq; i += kPgChunkThreads) {
+            children[i] = 0;
+            whole[i] = min(max(a.ctx_lens[i], 0), cap) / a.block_size;
+        }
         __syncthreads();
         for (int i = tid; i < a.n_seq; i += kPgChunkThreads) {
             const int p = a.parents[i];
             if ((unsigned)p < (unsigned)a.n_seq) atomicAdd(&children[p], 1);
         }
         __syncthreads();
-        const int64_t entries = (int64_t)a.n_seq * a.max_blocks;
-        for (int64_t i = tid; i < entries; i += kPgChunkThreads) {
-            const int v = a.tables[i] - b0;
-            if ((unsigned)v >= (unsigned)n) continue;
-            const int p = (int)(i / a.max_blocks), e = (int)(i - (int64_t)p * a.max_blocks);
-            const int kids = children[p], whole = min(max(a.ctx_lens[p], 0), cap) / a.block_size;
-            const int change = (e < whole ? kids : (kids > 0 ? 1 : 0)) - 1;
-            if (change) atomicAdd(&count[v], change);
+        constexpr int G = 8;                           // table entries in flight per thread
+        const int entries = a.n_seq * a.max_blocks;
+        for (int i0 = tid; i0 < entries; i0 += G * kPgChunkThreads) {
+            int v[G];
+#pragma unroll
+            for (int g = 0; g < G; g++) v[g] = a.tables[min(i0 + g * kPgChunkThreads, entries - 1)] - b0;
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                const int i = i0 + g * kPgChunkThreads;
+                if (i >= entries || (unsigned)v[g] >= (unsigned)n) continue;
+                const int p = (int)(__umulhi(2u * (uint32_t)i, a.row_mul) >> a.row_shift), e = i - p * a.max_blocks, kids = children[p];
+                const int change = (e < whole[p] ? kids : (kids > 0 ? 1 : 0)) - 1;
+                if (change) atomicAdd(&count[v[g]], change);
+            }
         }
         __syncthreads();
         const int per = (n + kPgChunkThreads - 1) / kPgChunkThreads, i0 = min(tid * per, n), i1 = min(i0 + per, n);
@@ -236,10 +247,17 @@ __global__ __launch_bounds__(kPgChunkThreads) void compact_plan_kernel(CompactAr
     __shared__ int red[kPgChunkThreads / kWave];
     const int tid = threadIdx.x, b0 = blockIdx.x * a.chunk, n = min(a.chunk, a.n_blocks - b0);
     int before = 0, all = 0;
-    for (int i = tid; i < a.n_blocks; i += kPgChunkThreads) {
-        const int used = a.ref[i] > 0;
-        all += used;
-        before += i < b0 ? used : 0;
+    constexpr int G = 8;                               // counts in flight per thread
+    for (int i0 = tid; i0 < a.n_blocks; i0 += G * kPgChunkThreads) {
+        int v[G];
+#pragma unroll
+        for (int g = 0; g < G; g++) v[g] = a.ref[min(i0 + g * kPgChunkThreads, a.n_blocks - 1)];
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            const int i = i0 + g * kPgChunkThreads, used = i < a.n_blocks && v[g] > 0;
+            all += used;
+            before += i < b0 ? used : 0;
+        }
     }
     before = pg_block_sum(before, red, kPgChunkThreads);
     all = pg_block_sum(all, red, kPgChunkThreads);
@@ -343,8 +361,9 @@ extern "C" int feather_paged_cache_fork(const void *const *caches_host, int64_t 
     if (rc != FEATHER_OK) return rc;
     FEATHER_CHECK(n_seq >= 0 && max_blocks >= 0 && block_size > 0, FEATHER_EINVAL, "%s: bad shape", me);
     FEATHER_CHECK(n_seq <= kPgMaxSlots, FEATHER_ESHAPE, "%s: n_seq=%lld above %d", me, (long long)n_seq, kPgMaxSlots);
-    FEATHER_CHECK(max_blocks < (1ll << 30) && block_size < (1ll << 30) && max_blocks * block_size < (1ll << 30), FEATHER_ESHAPE,
-                  "%s: shape too large", me);
+    FEATHER_CHECK(max_blocks < (1ll << 30) && block_size < (1ll << 30) && max_blocks * block_size < (1ll << 30) &&
+                      n_seq * max_blocks < (1ll << 30),
+                  FEATHER_ESHAPE, "%s: shape too large", me);
     FEATHER_CHECK(ref_counts && ref_out && scratch && ref_counts != ref_out, FEATHER_EINVAL, "%s: null pointer, or ref_out is ref_counts", me);
     FEATHER_CHECK(n_seq == 0 || (ctx_lens && parents && ctx_out && ctx_out != ctx_lens), FEATHER_EINVAL,
                   "%s: null pointer, or ctx_out is ctx_lens", me);
@@ -360,9 +379,12 @@ extern "C" int feather_paged_cache_fork(const void *const *caches_host, int64_t 
     a.need = (int32_t *)scratch; a.source = a.need + n_seq; a.free_count = a.source + n_seq; a.free_ids = a.free_count + kPgMaxChunks;
     a.n_seq = (int)n_seq; a.max_blocks = (int)max_blocks; a.block_size = (int)block_size; a.n_blocks = (int)n_blocks;
     a.chunk = (int)pg_chunk(n_blocks); a.chunks = (int)((n_blocks + a.chunk - 1) / a.chunk);
-    const size_t lds = ((size_t)a.chunk + n_seq) * 4;
+    const size_t lds = ((size_t)a.chunk + 2 * n_seq) * 4;
+    a.row_shift = 0;
+    while ((1ll << a.row_shift) < max_blocks) a.row_shift++;
+    a.row_mul = max_blocks > 0 ? (uint32_t)((1ull << (31 + a.row_shift)) / (uint64_t)max_blocks + 1) : 0;
     static unsigned long long lds_raised = 0;
-    hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(fork_plan_kernel), (size_t)(kPgMaxChunk + kPgMaxSlots) * 4, lds_raised);
+    hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(fork_plan_kernel), (size_t)(kPgMaxChunk + 2 * kPgMaxSlots) * 4, lds_raised);
     FEATHER_CHECK(e == hipSuccess, FEATHER_ELAUNCH, "%s: cannot raise LDS limit: %s", me, hipGetErrorString(e));
     hipStream_t s = (hipStream_t)stream;
     hipLaunchKernelGGL(fork_plan_kernel, dim3((unsigned)(a.chunks + n_seq)), dim3(kPgChunkThreads), lds, s, a);

@@ -155,7 +155,7 @@ __device__ __forceinline__ void chunk_fill_outside(const ChunkArgs &a, int part,
 
 constexpr int kChunkFillGroups = 8;    // workgroups of a grid that only look after rows outside every sequence
 constexpr int kChunkMinKeys = 256;     // a key range is not cut below this (LDS kernel / narrow kernel)
-constexpr int kNarrowMinKeys = 256;
+constexpr int kNarrowMinKeys = 512;
 constexpr int kNarrowStep = 128;       // keys that the four waves of a narrow workgroup take per turn
 
 // Least keys per range of the narrow kernel: the keys of all its tiles shared out evenly over the workgroups that the

@@ -112,16 +112,16 @@ def paged_chunk_attention_fp8_acc_fp32_gpu(q: torch.Tensor, k_cache: torch.Tenso
         raise ValueError(f"n_q_heads={n_q_heads} must be a multiple of n_kv_heads={n_kv_heads}")
     if n_blocks < 1 or block_size < 1:
         raise ValueError("the cache must hold at least one block")
-    for name, t, dims in (("block_tables", block_tables, 2), ("cu_seqlens", cu_seqlens, 1), ("ctx_lens", ctx_lens, 1)):
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != dims:
-            raise ValueError(f"{name} must be a {dims}-D int32 tensor")
-        if t.device != q.device:
-            raise ValueError(f"{name} is on {t.device}, q on {q.device}")
-    n_seq = ctx_lens.shape[0]
-    if block_tables.shape[0] != n_seq or cu_seqlens.shape[0] != n_seq + 1:
+    for name, t in (("block_tables", block_tables), ("cu_seqlens", cu_seqlens), ("ctx_lens", ctx_lens)):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+            raise ValueError(f"{name} must be an int32 tensor")
+    n_seq = ctx_lens.numel()
+    if ctx_lens.dim() != 1 or block_tables.dim() != 2 or block_tables.shape[0] != n_seq or cu_seqlens.shape != (n_seq + 1,):
         raise ValueError("block_tables must be [n_seq, max_blocks], cu_seqlens [n_seq + 1] and ctx_lens [n_seq]")
-    if k_cache.device != q.device or v_cache.device != q.device:
-        raise ValueError("q and the caches must be on the same device")
+    dev = q.device
+    if (k_cache.device != dev or v_cache.device != dev or block_tables.device != dev or cu_seqlens.device != dev
+            or ctx_lens.device != dev):
+        raise ValueError("q, the caches, block_tables, cu_seqlens and ctx_lens must be on the same device")
     if scale is None:
         scale = 1.0 / math.sqrt(d)
     if not 0 < scale < math.inf:
@@ -135,17 +135,18 @@ def paged_chunk_attention_fp8_acc_fp32_gpu(q: torch.Tensor, k_cache: torch.Tenso
     shape = (total, n_q_heads * dw) if kind == N.CHUNK_OUT_PACKED else (total, n_q_heads, d)
     fill = 1 if out is None else 0
     if out is None:
-        out = torch.empty(shape, dtype=out_dtype, device=q.device)
+        out = q.new_empty(shape, dtype=out_dtype)
     elif (not isinstance(out, torch.Tensor) or out.dtype != out_dtype or tuple(out.shape) != shape
-          or out.device != q.device or not out.is_contiguous()):
-        raise ValueError(f"out must be a contiguous {out_dtype} tensor of shape {shape} on {q.device}")
+          or out.device != dev or not out.is_contiguous()):
+        raise ValueError(f"out must be a contiguous {out_dtype} tensor of shape {shape} on {dev}")
     block_tables, cu_seqlens, ctx_lens = block_tables.contiguous(), cu_seqlens.contiguous(), ctx_lens.contiguous()
     max_blocks = block_tables.shape[1]
-    nbytes = N.lib().feather_paged_chunk_attn_scratch_bytes(n_seq, total, n_q_heads, n_kv_heads, d, max_blocks * block_size,
+    lib = N.lib()
+    nbytes = lib.feather_paged_chunk_attn_scratch_bytes(n_seq, total, n_q_heads, n_kv_heads, d, max_blocks * block_size,
                                                             max_q_len)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes > 0 else None
-    N.call(q.device, "feather_paged_chunk_attn_fp8", N.ptr(q), N.ptr(k_cache), N.ptr(v_cache), N.ptr(block_tables),
-           N.ptr(cu_seqlens), N.ptr(ctx_lens), N.ptr(out), kind, fill, N.ptr(scratch) if scratch is not None else None,
+    scratch = q.new_empty(nbytes // 4) if nbytes > 0 else None
+    N.call(dev, "feather_paged_chunk_attn_fp8", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(),
+           cu_seqlens.data_ptr(), ctx_lens.data_ptr(), out.data_ptr(), kind, fill, scratch.data_ptr() if scratch is not None else None,
            max(nbytes, 0), n_seq, total, n_q_heads, n_kv_heads, d, block_size, max_blocks, n_blocks, max_q_len,
            1 if causal else 0, code, float(scale))
     return out

@@ -9,6 +9,7 @@ tables, lengths and counts; the caches are updated in place, in blocks that were
 from __future__ import annotations
 
 import ctypes
+import operator
 
 import torch
 
@@ -20,36 +21,43 @@ __all__ = ["paged_cache_fork", "paged_cache_compact"]
 def _index(t: torch.Tensor, name: str, shape=None) -> torch.Tensor:
     if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or not t.is_cuda:
         raise ValueError(f"{name} must be an int32 tensor on the device")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     return t.contiguous()
 
 
+_dtype, _shape = operator.attrgetter("dtype"), operator.attrgetter("shape")
+
+
 def _pool(caches, ref_counts: torch.Tensor):
-    """Checks the caches against the pool; returns their pointers as a C array, the bytes and the tokens of a block."""
-    caches = list(caches)
+    """Checks the caches against the pool; returns their pointers as a C array, how many, and the bytes and tokens of a
+    block.  (A decoder has dozens of caches: every check is one pass in C over all of them.)"""
+    caches = tuple(caches)
     if not caches:
         raise ValueError("caches must hold at least one cache tensor")
-    first = caches[0]
-    for i, t in enumerate(caches):
-        N.as_words(t, f"caches[{i}]")
-        if t.dim() != 4 or not t.is_contiguous():
-            raise ValueError(f"caches[{i}] is updated in place: expected a contiguous [n_blocks, n_kv_heads, block_size, d/4]")
-        if t.shape != first.shape or t.device != first.device:
-            raise ValueError("all caches must have the same shape and device")
-        if t.data_ptr() % 16 != 0:
-            raise ValueError(f"caches[{i}] must be 16-byte aligned")
-    ptrs = [t.data_ptr() for t in caches]
+    first = N.as_words(caches[0], "caches[0]")
+    try:
+        devices, dtypes, shapes = set(map(torch.Tensor.get_device, caches)), set(map(_dtype, caches)), set(map(_shape, caches))
+        whole, ptrs = all(map(torch.Tensor.is_contiguous, caches)), list(map(torch.Tensor.data_ptr, caches))
+    except TypeError:
+        raise ValueError("caches must be tensors of packed words") from None
+    if len(devices) != 1 or len(shapes) != 1:
+        raise ValueError("all caches must have the same shape and device")
+    if not dtypes.issubset(N._WORD_DTYPES):
+        raise ValueError(f"caches must be uint32/int32/float32 containers, got {dtypes}")
+    if not whole or first.dim() != 4:
+        raise ValueError("caches are updated in place: expected contiguous [n_blocks, n_kv_heads, block_size, d/4]")
     if len(set(ptrs)) != len(ptrs):
         raise ValueError("caches holds the same tensor twice")
-    block_bytes = 4 * first.shape[1] * first.shape[2] * first.shape[3]
+    n_blocks, n_kv, block_size, dw = first.shape
+    block_bytes = 4 * n_kv * block_size * dw
     if block_bytes == 0 or block_bytes % 16 != 0:
         raise ValueError(f"a block of {block_bytes} bytes is not a multiple of 16")
-    if ref_counts.shape != (first.shape[0],) or first.shape[0] < 1:
-        raise ValueError(f"ref_counts must be [n_blocks={first.shape[0]}] with at least one block")
+    if ref_counts.shape != (n_blocks,) or n_blocks < 1:
+        raise ValueError(f"ref_counts must be [n_blocks={n_blocks}] with at least one block")
     if ref_counts.device != first.device:
         raise ValueError("ref_counts and the caches must be on the same device")
-    return (ctypes.c_void_p * len(ptrs))(*ptrs), len(ptrs), block_bytes, first.shape[2]
+    return (ctypes.c_void_p * len(ptrs))(*ptrs), len(ptrs), block_bytes, block_size
 
 
 def paged_cache_fork(caches, block_tables: torch.Tensor, ctx_lens: torch.Tensor, ref_counts: torch.Tensor,
@@ -75,15 +83,14 @@ def paged_cache_fork(caches, block_tables: torch.Tensor, ctx_lens: torch.Tensor,
     if room is not None:
         room = _index(room, "room", (n_seq,))
     dev, n_blocks = ref_counts.device, ref_counts.shape[0]
-    for t in (block_tables, ctx_lens, parents, room):
-        if t is not None and t.device != dev:
-            raise ValueError("all tensors must be on the same device")
+    if block_tables.device != dev or ctx_lens.device != dev or parents.device != dev or (room is not None and room.device != dev):
+        raise ValueError("all tensors must be on the same device")
     tables_out, ctx_out, ref_out = torch.empty_like(block_tables), torch.empty_like(ctx_lens), torch.empty_like(ref_counts)
     status = torch.empty_like(ctx_lens)
-    scratch = torch.empty(N.lib().feather_paged_cache_fork_scratch_bytes(n_seq, n_blocks), dtype=torch.uint8, device=dev)
-    N.call(dev, "feather_paged_cache_fork", ctypes.addressof(ptrs), n_caches, block_bytes, N.ptr(block_tables),
-           N.ptr(ctx_lens), N.ptr(ref_counts), N.ptr(parents), N.ptr(room) if room is not None else None,
-           N.ptr(tables_out), N.ptr(ctx_out), N.ptr(ref_out), N.ptr(status), N.ptr(scratch), n_seq, max_blocks,
+    scratch = ref_counts.new_empty(N.lib().feather_paged_cache_fork_scratch_bytes(n_seq, n_blocks) // 4)
+    N.call(dev, "feather_paged_cache_fork", ctypes.addressof(ptrs), n_caches, block_bytes, block_tables.data_ptr(),
+           ctx_lens.data_ptr(), ref_counts.data_ptr(), parents.data_ptr(), room.data_ptr() if room is not None else None,
+           tables_out.data_ptr(), ctx_out.data_ptr(), ref_out.data_ptr(), status.data_ptr(), scratch.data_ptr(), n_seq, max_blocks,
            block_size, n_blocks)
     return tables_out, ctx_out, ref_out, status
 
@@ -102,9 +109,9 @@ def paged_cache_compact(caches, block_tables: torch.Tensor, ref_counts: torch.Te
     if block_tables.device != dev:
         raise ValueError("all tensors must be on the same device")
     tables_out, ref_out, block_map = torch.empty_like(block_tables), torch.empty_like(ref_counts), torch.empty_like(ref_counts)
-    n_live = torch.empty((1,), dtype=torch.int32, device=dev)
-    scratch = torch.empty(N.lib().feather_paged_cache_compact_scratch_bytes(n_blocks), dtype=torch.uint8, device=dev)
-    N.call(dev, "feather_paged_cache_compact", ctypes.addressof(ptrs), n_caches, block_bytes, N.ptr(block_tables),
-           N.ptr(ref_counts), N.ptr(tables_out), N.ptr(ref_out), N.ptr(block_map), N.ptr(n_live), N.ptr(scratch),
+    n_live = ref_counts.new_empty(1)
+    scratch = ref_counts.new_empty(N.lib().feather_paged_cache_compact_scratch_bytes(n_blocks) // 4)
+    N.call(dev, "feather_paged_cache_compact", ctypes.addressof(ptrs), n_caches, block_bytes, block_tables.data_ptr(),
+           ref_counts.data_ptr(), tables_out.data_ptr(), ref_out.data_ptr(), block_map.data_ptr(), n_live.data_ptr(), scratch.data_ptr(),
            block_tables.numel(), n_blocks)
     return tables_out, ref_out, block_map, n_live

@@ -20,7 +20,7 @@ __all__ = ["quant_pack_f32", "add_rmsnorm_pack", "rope_append", "rope_append_chu
 def _f32(t: torch.Tensor, name: str, shape=None) -> torch.Tensor:
     if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or not t.is_cuda or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous float32 tensor on the device")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != torch.Size(shape):
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     return t
 
@@ -168,10 +168,8 @@ def rope_append_chunk(qkv: torch.Tensor, cu_seqlens: torch.Tensor, start_pos: to
     code = N.mode_code(mode)
     if layout not in _ROPE_LAYOUTS:
         raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}")
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        N.as_words(t, name)
-        if not t.is_contiguous():
-            raise ValueError(f"{name} is written in place and must be contiguous")
+    if N.as_words(k_cache, "k_cache") is not k_cache or N.as_words(v_cache, "v_cache") is not v_cache:
+        raise ValueError("k_cache and v_cache are written in place and must be contiguous")
     if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
         raise ValueError("expected k_cache/v_cache [n_blocks, n_kv_heads, block_size, d/4]")
     n_blocks, n_kv, block_size, dw = k_cache.shape
@@ -184,11 +182,11 @@ def rope_append_chunk(qkv: torch.Tensor, cu_seqlens: torch.Tensor, start_pos: to
     if qkv.dim() != 2 or qkv.shape[1] != heads * d:
         raise ValueError(f"qkv must be [total_rows, {heads * d}], got {tuple(qkv.shape)}")
     total = qkv.shape[0]
-    if total > 1 and (qkv.stride(1) != 1 or qkv.stride(0) % 4 != 0 or qkv.stride(0) < heads * d) or qkv.data_ptr() % 16 != 0:
-        qkv = qkv.contiguous() if qkv.data_ptr() % 16 == 0 else qkv.clone(memory_format=torch.contiguous_format)
-    row_stride = qkv.stride(0) if total > 1 else heads * d
-    if qkv.stride(1) != 1:
-        qkv, row_stride = qkv.contiguous(), heads * d
+    if not qkv.is_contiguous() and (qkv.stride(1) != 1 or qkv.stride(0) % 4 != 0 or qkv.stride(0) < heads * d):
+        qkv = qkv.contiguous()
+    if qkv.data_ptr() % 16 != 0:
+        qkv = qkv.clone(memory_format=torch.contiguous_format)
+    row_stride = heads * d if qkv.is_contiguous() else qkv.stride(0)
     _i32(cu_seqlens, "cu_seqlens")
     n_seq = cu_seqlens.numel() - 1
     if cu_seqlens.dim() != 1 or n_seq < 0:
@@ -204,16 +202,17 @@ def rope_append_chunk(qkv: torch.Tensor, cu_seqlens: torch.Tensor, start_pos: to
         raise ValueError(f"rot_dim={rot} (two per frequency) must be a multiple of 8 and at most the head dim {d}")
     if not math.isfinite(amplitude):
         raise ValueError(f"amplitude must be finite, got {amplitude}")
-    _same_device(qkv, cu_seqlens, start_pos, block_tables, k_cache, v_cache, freq)
     dev = qkv.device
-    qp = torch.empty((total, n_q, dw), dtype=torch.uint32, device=dev)
-    ctx_after = torch.empty((n_seq,), dtype=torch.int32, device=dev)
-    status = torch.empty((n_seq,), dtype=torch.int32, device=dev)
+    if (k_cache.device != dev or v_cache.device != dev or cu_seqlens.device != dev or start_pos.device != dev
+            or block_tables.device != dev or freq.device != dev):
+        raise ValueError("all tensors must be on the same device")
+    qp = qkv.new_empty((total, n_q, dw), dtype=torch.uint32)
+    ctx_after, status = torch.empty_like(start_pos), torch.empty_like(start_pos)
     rotated = torch.empty((total, heads, d), dtype=torch.float32, device=dev) if return_f32 else None
-    N.call(dev, "feather_rope_append_chunk", N.ptr(qkv), 1 if qkv.dtype == torch.float16 else 0, row_stride,
-           N.ptr(cu_seqlens), N.ptr(start_pos), N.ptr(block_tables), N.ptr(freq), float(amplitude), rot,
-           _ROPE_LAYOUTS[layout], N.ptr(qp), N.ptr(k_cache), N.ptr(v_cache), N.ptr(ctx_after), N.ptr(status),
-           N.ptr(rotated) if rotated is not None else None, 1, n_seq, total, n_q, n_kv, d, block_size,
+    N.call(dev, "feather_rope_append_chunk", qkv.data_ptr(), 1 if qkv.dtype == torch.float16 else 0, row_stride,
+           cu_seqlens.data_ptr(), start_pos.data_ptr(), block_tables.data_ptr(), freq.data_ptr(), float(amplitude), rot,
+           _ROPE_LAYOUTS[layout], qp.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), ctx_after.data_ptr(), status.data_ptr(),
+           rotated.data_ptr() if rotated is not None else None, 1, n_seq, total, n_q, n_kv, d, block_size,
            block_tables.shape[1], n_blocks, code)
     res = (qp, ctx_after, status)
     return res + (rotated,) if return_f32 else res
