@@ -33,8 +33,8 @@ struct ChunkArgs {
     float *part;            // partial results of the LDS kernel's key ranges (z_wide > 1), then the (maximum, sum) pairs
     int n_seq, total_rows, n_q_heads, n_kv_heads, group, block_size, max_blocks;
     uint32_t max_blk;       // last block of the cache: an entry outside the cache is read as this one
-    uint32_t div_mul, group_mul, kv_mul;   // x / size = umulhi(2 x, mul) >> shift for 0 <= x < 2^31 (block_size, group, n_kv_heads)
-    int div_shift, group_shift, kv_shift;
+    uint32_t div_mul, group_mul, kv_mul, head_mul;   // x / size = umulhi(2 x, mul) >> shift for 0 <= x < 2^31 (block_size, group, n_kv_heads, n_q_heads)
+    int div_shift, group_shift, kv_shift, head_shift;
     int causal, out_kind, fill;
     int z_wide, z_narrow;             // most key ranges of a tile in either kernel
     float per_group;                  // KV heads over the workgroups of the narrow kernel that the chip holds at once
@@ -1344,7 +1344,7 @@ __global__ __launch_bounds__(256, (D / 64) * NB <= 4 ? 2 : 1) void chunk_narrow_
 constexpr int kMergeSeqs = 1024;
 
 template <int D, int MODE>
-__global__ __launch_bounds__(256) void chunk_merge_kernel(ChunkArgs a, int qt_wide, int bn_wide, int qt_narrow, int zl) {
+__global__ __launch_bounds__(256) void chunk_merge_kernel(ChunkArgs a, int qt_wide_log2, int bn_wide, int qt_narrow_log2, int zl_log2) {
     constexpr int DW = D / 4, G = 4;
     __shared__ float4_t x_lds[256];
     __shared__ float2p_t ml_lds[256];
@@ -1354,16 +1354,16 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(ChunkArgs a, int qt_wi
         for (int s = threadIdx.x; s <= a.n_seq; s += 256) cu_lds[s] = chunk_clamp_row(a.cu_seqlens[s], a.total_rows);
     __syncthreads();
     auto cu_at = [&](int s) { return cached ? cu_lds[s] : chunk_clamp_row(a.cu_seqlens[s], a.total_rows); };
-    const int tid = threadIdx.x, w4 = tid % DW, zi = (tid / DW) % zl;
-    const int64_t items = (int64_t)a.total_rows * a.n_q_heads;
-    const int64_t item = (int64_t)blockIdx.x * (256 / (DW * zl)) + tid / (DW * zl);
+    const int tid = threadIdx.x, zl = 1 << zl_log2, w4 = tid % DW, zi = (tid / DW) & (zl - 1);
+    const int items = a.total_rows * a.n_q_heads;           // below 2^30
+    const int item = (int)blockIdx.x * ((256 / DW) >> zl_log2) + ((tid / DW) >> zl_log2);
     int used = 0;
     bool zero = false;
     const float *part = a.part;                        // partial results of the row's kernel: [range][item][D], [range][item] pairs
     int64_t part_items = items, part_item = item;
     int z = 1;
     if (item < items) {
-        const int row = (int)(item / a.n_q_heads), head = (int)(item % a.n_q_heads);
+        const int row = (int)(__umulhi(2u * (uint32_t)item, a.head_mul) >> a.head_shift), head = item - row * a.n_q_heads;
         int lo = 0, hi = a.n_seq;                      // last sequence that starts at or before the row
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
@@ -1376,10 +1376,10 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(ChunkArgs a, int qt_wi
             const int ctx = min(max(a.ctx_lens[lo], 0), a.max_blocks * a.block_size), p0 = ctx - (r1 - r0);
             const int cols = (r1 - r0) * a.group;
             const bool narrow = cols <= a.col_split;
-            const int qt = narrow ? (a.narrow_rows ? kAnyColumns : qt_narrow) : qt_wide;
+            const int qt_log2 = narrow ? qt_narrow_log2 : qt_wide_log2;
             z = narrow ? a.z_narrow : a.z_wide;
-            const int col0 = ((row - r0) * a.group + head % a.group) / qt * qt;
-            const int keys = a.causal ? max(p0 + chunk_row_of(a, min(col0 + qt, cols) - 1) + 1, 0) : ctx;
+            const int col = (row - r0) * a.group + head - chunk_row_of(a, head) * a.group, col_end = ((col >> qt_log2) + 1) << qt_log2;   // of its tile
+            const int keys = a.causal ? max(p0 + chunk_row_of(a, min(col_end, cols) - 1) + 1, 0) : ctx;
             if (z > 1) {
                 if (narrow) {
                     part = a.part_narrow;
@@ -1461,6 +1461,8 @@ static constexpr int ring_steps(int d, int nb) { return d == 64 ? 4 : (d == 128 
 
 constexpr int kWide64Blocks = 2;   // 32-column blocks of a wave of the d = 64 kernel (256 columns per workgroup)
 
+static int log2_of(int64_t x) { int l = 0; while ((1ll << l) < x) l++; return l; }
+
 static int wide_columns(int64_t d) { return d == 64 ? 256 : (d == 512 ? 64 : 128); }
 static int narrow_most_blocks(int64_t d) { return d <= 128 ? 4 : (d == 256 ? 2 : 1); }
 
@@ -1487,9 +1489,12 @@ static ChunkPlan chunk_plan(int64_t n_seq, int64_t total_rows, int64_t n_q_heads
         p.col_split = kAnyColumns;
         p.nb = cols <= 16 ? 1 : (cols <= 32 ? 2 : 4);
     } else {
-        p.narrow = n_seq > 1 && rows_most * n_seq > total_rows;   // the lengths differ: some may be short
         p.wide = true;
         p.nb = narrow_most_blocks(d) >= 2 ? 2 : 1;
+        // with n_seq - 1 sequences of the longest length, can the last one be short?  (If the hint is wrong the LDS kernel
+        // takes the short ones too.)
+        const int64_t least = total_rows - (n_seq - 1) * rows_most;
+        p.narrow = n_seq > 1 && (least < 0 ? 0 : least) * group <= 16 * p.nb;
         p.col_split = p.narrow ? 16 * p.nb : 0;
     }
     p.narrow_rows = p.wide && p.narrow ? (int)(p.col_split / group) : 0;
@@ -1565,11 +1570,11 @@ static int launch_chunk(const ChunkArgs &a, const ChunkPlan &p, hipStream_t s) {
     }
     if (rc != FEATHER_OK || !merge) return rc;
     constexpr int DW = D / 4;
-    int zl = 1;                                              // four ranges per thread and turn; rows of the LDS kernel have few
-    while (!p.wide && zl * 4 < a.z_narrow && zl * DW < 256) zl *= 2;
-    const int64_t per_group = 256 / (DW * zl), items = (int64_t)a.total_rows * a.n_q_heads;
+    int zl = 0;                                              // four ranges per thread and turn; rows of the LDS kernel have few
+    while (!p.wide && (4 << zl) < a.z_narrow && (DW << zl) < 256) zl++;
+    const int64_t per_group = (256 / DW) >> zl, items = (int64_t)a.total_rows * a.n_q_heads;
     hipLaunchKernelGGL((chunk_merge_kernel<D, MODE>), dim3((unsigned)((items + per_group - 1) / per_group)), dim3(256), 0, s, a,
-                       wide_columns(D), D == 512 ? 32 : 64, 16 * p.nb, zl);
+                       log2_of(wide_columns(D)), D == 512 ? 32 : 64, log2_of(16 * p.nb), zl);
     return check_launch("feather_paged_chunk_attn_fp8 (merge of the key ranges)");
 }
 
@@ -1645,6 +1650,7 @@ extern "C" int feather_paged_chunk_attn_fp8(const void *q, const void *k_cache, 
     divisor(block_size, a.div_mul, a.div_shift);
     divisor(n_q_heads / n_kv_heads, a.group_mul, a.group_shift);
     divisor(n_kv_heads, a.kv_mul, a.kv_shift);
+    divisor(n_q_heads, a.head_mul, a.head_shift);
     a.q = (const uint32_t *)q; a.k_cache = (const uint32_t *)k_cache; a.v_cache = (const uint32_t *)v_cache;
     a.block_tables = (const int32_t *)block_tables; a.cu_seqlens = (const int32_t *)cu_seqlens; a.ctx_lens = (const int32_t *)ctx_lens;
     a.out = out; a.part = (float *)scratch;

@@ -50,10 +50,10 @@ __device__ void rope_chunk_status(const RopeChunkArgs &a, int s) {
 template <bool F16>
 __device__ __forceinline__ float4_t rope_load4(const void *p, int64_t at) {
     if constexpr (F16) {
-        const half4_t h = *reinterpret_cast<const half4_t *>(static_cast<const _Float16 *>(p) + at);
+        const half4_t h = __builtin_nontemporal_load(reinterpret_cast<const half4_t *>(static_cast<const _Float16 *>(p) + at));
         return float4_t{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
     } else {
-        return *reinterpret_cast<const float4_t *>(static_cast<const float *>(p) + at);
+        return __builtin_nontemporal_load(reinterpret_cast<const float4_t *>(static_cast<const float *>(p) + at));
     }
 }
 
@@ -175,8 +175,13 @@ __global__ __launch_bounds__(kRcThreads) void rope_chunk_kernel(RopeChunkArgs a,
             const int kvh = head[i] - a.n_q - (is_k ? 0 : a.n_kv);
             dst = (is_k ? a.k_cache : a.v_cache) + (slot + (int64_t)kvh * a.block_size) * (a.d / 4);
         }
-        dst[at_lo[i] / 4] = quant4<MODE>(lo[i][0], lo[i][1], lo[i][2], lo[i][3]);
-        dst[at_hi[i] / 4] = quant4<MODE>(hi[i][0], hi[i][1], hi[i][2], hi[i][3]);
+        const uint32_t wlo = quant4<MODE>(lo[i][0], lo[i][1], lo[i][2], lo[i][3]), whi = quant4<MODE>(hi[i][0], hi[i][1], hi[i][2], hi[i][3]);
+        if (at_hi[i] == at_lo[i] + 4) {               // neighbours (8 bytes from a multiple of 8 on: d is one)
+            *reinterpret_cast<u32x2 *>(dst + at_lo[i] / 4) = u32x2{wlo, whi};
+        } else {
+            dst[at_lo[i] / 4] = wlo;
+            dst[at_hi[i] / 4] = whi;
+        }
     }
 }
 
@@ -211,7 +216,7 @@ extern "C" int feather_rope_append_chunk(const void *qkv, int src_f16, int64_t r
     FEATHER_CHECK(cu_seqlens && (n_seq == 0 || (start_pos && ctx_after && (block_tables || max_blocks == 0))) && (freq_f64 || rot_dim == 0), FEATHER_EINVAL,
                   "%s: null pointer", me);
     FEATHER_CHECK(total_rows == 0 || (qkv && (q_packed || n_q_heads == 0) && k_cache && v_cache), FEATHER_EINVAL, "%s: null pointer", me);
-    FEATHER_CHECK(aligned(qkv, src_f16 ? 8 : 16) && aligned(q_packed, 4) && aligned(k_cache, 4) && aligned(v_cache, 4) &&
+    FEATHER_CHECK(aligned(qkv, src_f16 ? 8 : 16) && aligned(q_packed, 8) && aligned(k_cache, 8) && aligned(v_cache, 8) &&
                       aligned(rot_f32, 16) && aligned(freq_f64, 8) && aligned(cu_seqlens, 4) && aligned(start_pos, 4) &&
                       aligned(block_tables, 4) && aligned(ctx_after, 4) && aligned(seq_status, 4),
                   FEATHER_EINVAL, "%s: misaligned pointer", me);
@@ -224,14 +229,22 @@ extern "C" int feather_rope_append_chunk(const void *qkv, int src_f16, int64_t r
     a.block_size = (int)block_size; a.max_blocks = (int)max_blocks; a.n_blocks = (int)n_blocks;
     a.interleaved = layout == FEATHER_ROPE_INTERLEAVED; a.fill = fill; a.amplitude = amplitude;
     const int64_t units = heads * (d / 8);
-    constexpr int U = 2;
+    const int U = units <= kRcThreads ? 1 : (units <= 2 * kRcThreads ? 2 : (units <= 3 * kRcThreads ? 3 : 4));
     const int64_t parts = (units + U * kRcThreads - 1) / (U * kRcThreads);
     const int64_t grid = n_seq + total_rows * parts;
     FEATHER_CHECK(grid < (1ll << 31), FEATHER_ESHAPE, "%s: grid too large", me);
-#define FEATHER_RC(MM, FF)                                                                                             \
-    hipLaunchKernelGGL((rope_chunk_kernel<MM, FF, U>), dim3((unsigned)grid), dim3(kRcThreads), 0, (hipStream_t)stream, a, (int)parts)
-    if (mode == FEATHER_E5M2) { if (src_f16) FEATHER_RC(FEATHER_E5M2, true); else FEATHER_RC(FEATHER_E5M2, false); }
-    else { if (src_f16) FEATHER_RC(FEATHER_E4M3, true); else FEATHER_RC(FEATHER_E4M3, false); }
+#define FEATHER_RC(MM, FF, UU)                                                                                         \
+    hipLaunchKernelGGL((rope_chunk_kernel<MM, FF, UU>), dim3((unsigned)grid), dim3(kRcThreads), 0, (hipStream_t)stream, a, (int)parts)
+#define FEATHER_RCU(MM, FF)                                                                                            \
+    do {                                                                                                               \
+        if (U == 1) FEATHER_RC(MM, FF, 1);                                                                             \
+        else if (U == 2) FEATHER_RC(MM, FF, 2);                                                                        \
+        else if (U == 3) FEATHER_RC(MM, FF, 3);                                                                        \
+        else FEATHER_RC(MM, FF, 4);                                                                                    \
+    } while (0)
+    if (mode == FEATHER_E5M2) { if (src_f16) FEATHER_RCU(FEATHER_E5M2, true); else FEATHER_RCU(FEATHER_E5M2, false); }
+    else { if (src_f16) FEATHER_RCU(FEATHER_E4M3, true); else FEATHER_RCU(FEATHER_E4M3, false); }
+#undef FEATHER_RCU
 #undef FEATHER_RC
     return check_launch(me);
 }

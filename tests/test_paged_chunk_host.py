@@ -58,7 +58,10 @@ def test_rope_chunk_argument_checks():
                 dict(mb=1 << 30, bs=4), dict(total=1 << 30)):
         assert call(**bad) == N.ESHAPE, bad
     assert call(n_seq=0, total=0) == N.OK
-    assert call(p=(8, 4, 4, 4, 8, 4, 4, 4, 4, 4, 16)) == N.EINVAL and b"misaligned" in L.feather_last_error()
+    assert call(p=(8, 4, 4, 4, 8, 8, 8, 8, 4, 4, 16)) == N.EINVAL and b"misaligned" in L.feather_last_error()
+
+
+    assert call(p=(16, 4, 4, 4, 8, 8, 8, 4, 4, 4, 16)) == N.EINVAL                   # words of a row are stored in pairs
 
 
 def test_cache_pool_argument_checks():
