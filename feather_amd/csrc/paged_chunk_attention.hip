@@ -514,7 +514,7 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn_kernel(ChunkArgs a
     }
 }
 
-// ---- d = 64: tiles through LDS on the 32x32 matrix instructions ---------------------------------------------------------
+// ---- tiles through LDS on the 32x32 matrix instructions -----------------------------------------------------------------
 // The split and the numerics of chunk_attn_kernel, and the instruction mix of the prefill kernel's d = 64 form: vector
 // issue bounds this head dim, and an instruction of 32x32 holds it half as long per product as two of 16x16 --
 //     S^T[32 keys, 32 cols] = v_mfma_f32_32x32x64_f8f6f4 (E5M2 bytes as they are: the whole head dim) or four of
@@ -525,15 +525,17 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn_kernel(ChunkArgs a
 // PAGE16 (block_size % 16 == 0): the 16 keys that a wave stages share a block, whose address is then scalar.
 typedef int int8p_t __attribute__((ext_vector_type(8)));
 
-template <int MODE, int CB, int WAVES, int OCC, bool PAGE16, bool ZS>
-__global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn64_kernel(ChunkArgs a, int n_slots) {
-    constexpr int D = 64, DW = 16, BN = 64;
+template <int D, int MODE, int CB, int WAVES, int OCC, bool PAGE16, bool ZS>
+__global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn32_kernel(ChunkArgs a, int n_slots) {
     constexpr bool BF8 = MODE == FEATHER_E5M2;
+    constexpr int DW = D / 4, BN = 64, DB = D / 32, STEPS = BF8 ? D / 64 : D / 16;   // 32-dim blocks; matrix steps of a score block
     constexpr int KP = (BF8 ? D : 2 * D) + 16;   // K row pitch in LDS, bytes
     constexpr int VS = BN;                       // fp16 per V^T row
     constexpr int kThreads = 64 * WAVES, QT = 32 * CB * WAVES;
     constexpr int kBufBytes = BN * KP + D * VS * 2;
-    static_assert(kThreads >= 256, "256 threads stage a tile");
+    constexpr bool kSplit = D * 16 < 2 * kThreads;   // more threads than a tile has 16-byte units: half of the waves stage K, half V
+    constexpr int UNITS = BN * D / 16, STAGERS = kSplit ? kThreads / 2 : kThreads, NU = UNITS / STAGERS;
+    static_assert(UNITS % STAGERS == 0 && STAGERS % 64 == 0 && NU >= 1, "tile / workgroup mismatch");
 
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     auto swz = [](int row) { return ((row >> 1) & 7) ^ ((row >> 4) & 1); };   // 16-byte chunk c of V^T row r lives at chunk c ^ swz(r)
@@ -588,70 +590,79 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn64_kernel(ChunkArgs
     const int tile_first = a.causal ? t.p0 + chunk_row_of(a, t.col0) : t.ctx - 1;
     const bool wave_has = qc0 < t.cols;
 
-    int8p_t qf[BF8 ? CB : 1];
-    half8_t qh16[BF8 ? 1 : CB][BF8 ? 1 : 4];
+    int8p_t qf[BF8 ? CB : 1][BF8 ? STEPS : 1];
+    half8_t qh16[BF8 ? 1 : CB][BF8 ? 1 : STEPS];
 #pragma unroll
     for (int b = 0; b < CB; b++) {
-        if constexpr (BF8) {
-            const u32x2 *src = reinterpret_cast<const u32x2 *>(a.q + item[b] * DW + 8 * h);   // q need not be aligned to 16 bytes
-            const u32x2 w0 = src[0], w1 = src[1], w2 = src[2], w3 = src[3];
-            qf[b] = int8p_t{(int)w0.x, (int)w0.y, (int)w1.x, (int)w1.y, (int)w2.x, (int)w2.y, (int)w3.x, (int)w3.y};
-        } else {
 #pragma unroll
-            for (int st = 0; st < 4; st++) {
+        for (int st = 0; st < STEPS; st++) {
+            if constexpr (BF8) {
+                const u32x2 *src = reinterpret_cast<const u32x2 *>(a.q + item[b] * DW + 16 * st + 8 * h);   // q need not be aligned to 16 bytes
+                const u32x2 w0 = src[0], w1 = src[1], w2 = src[2], w3 = src[3];
+                qf[b][st] = int8p_t{(int)w0.x, (int)w0.y, (int)w1.x, (int)w1.y, (int)w2.x, (int)w2.y, (int)w3.x, (int)w3.y};
+            } else {
                 const u32x2 w = *reinterpret_cast<const u32x2 *>(a.q + item[b] * DW + 4 * st + 2 * h);
                 qh16[b][st] = chunk_dec8<MODE>(w.x, w.y);
             }
         }
     }
 
-    float16_t o[CB][2];                          // [32-dim block]
+    float16_t o[CB][DB];                         // [32-dim block]
     float m_run[CB], mc_run[CB], l_run[CB];      // reference point (raw, and times scale * log2 e), the lane's share of the sum
 #pragma unroll
     for (int b = 0; b < CB; b++) {
         m_run[b] = mc_run[b] = -INFINITY;
         l_run[b] = 0.f;
 #pragma unroll
-        for (int d = 0; d < 2; d++)
+        for (int d = 0; d < DB; d++)
 #pragma unroll
             for (int r = 0; r < 16; r++) o[b][d][r] = 0.f;
     }
 
-    // ---- staging: 256 threads carry V (4 keys x 4 dims each), 256 threads K (16 bytes of one key each): the same ones in a
-    // four-wave workgroup, waves 0-3 and 4-7 in an eight-wave one.  A wave's keys are 16 neighbours in both.
-    constexpr bool kSplit = kThreads >= 512;
-    const bool stages_v = tid < 256, stages_k = kSplit ? tid >= 256 : tid < 256;
-    const int kt = kSplit ? tid - 256 : tid;     // index among the K stagers
-    const int key16 = 16 * (wave & 3);           // the wave's first key inside a tile
+    // ---- staging: a thread carries NU units of K (16 bytes of one key) and of V (4 keys x 4 dims); unit u of either is in
+    // the keys u / (D / 16) .. of the tile, so the 64 units of a wave lie in 16 neighbouring keys, the same for K and V
+    const bool stages_v = !kSplit || wave < WAVES / 2, stages_k = !kSplit || wave >= WAVES / 2;
+    const int stager = kSplit && wave >= WAVES / 2 ? tid - STAGERS : tid;
+    const int key_wave = (kSplit ? wave % (WAVES / 2) : wave) * (1024 / D);   // the wave's first key of its first units
+    constexpr int kKeysPerTurn = STAGERS * 16 / D;
     const __attribute__((address_space(4))) int32_t *bt_const = (const __attribute__((address_space(4))) int32_t *)bt;   // read only while the kernel runs: scalar loads
-    int id_k = 0, id_v[4] = {0, 0, 0, 0};        // PAGE16: id_k only, wave-uniform
+    int id_k[NU], id_v[PAGE16 ? 1 : NU][PAGE16 ? 1 : 4];   // PAGE16: id_k only, wave-uniform
+    auto first16 = [&](int key0, int i) { return min((key0 + key_wave + kKeysPerTurn * i) & ~15, (key_end - 1) & ~15); };
     auto fetch_ids = [&](int key0) {
-        if constexpr (PAGE16) {
-            id_k = bt_const[chunk_block_of(a, min(key0 + key16, (key_end - 1) & ~15))];
-        } else {
-            if (stages_k) id_k = bt[chunk_block_of(a, min(key0 + kt / 4, key_end - 1))];
-            if (stages_v)
 #pragma unroll
-                for (int r = 0; r < 4; r++) id_v[r] = bt[chunk_block_of(a, min(key0 + 4 * (tid / DW) + r, key_end - 1))];
+        for (int i = 0; i < NU; i++) {
+            const int u = stager + STAGERS * i;
+            if constexpr (PAGE16) {
+                id_k[i] = bt_const[chunk_block_of(a, first16(key0, i))];
+            } else {
+                if (stages_k) id_k[i] = bt[chunk_block_of(a, min(key0 + u / (D / 16), key_end - 1))];
+                if (stages_v)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) id_v[i][r] = bt[chunk_block_of(a, min(key0 + 4 * (u / DW) + r, key_end - 1))];
+            }
         }
     };
-    u32x4 kreg;
-    uint32_t vreg[4];
+    u32x4 kreg[NU];
+    uint32_t vreg[NU][4];
     auto prefetch = [&](int key0) {              // keys past the end: another key's row (masked; its V is zeroed by `stage`)
-        if constexpr (PAGE16) {
-            const int pos = min(key0 + key16, (key_end - 1) & ~15);
-            if (stages_k) kreg = *reinterpret_cast<const u32x4 *>(row_at(a.k_cache, id_k, pos) + (uint32_t)((kt / 4 % 16) * D + 16 * (kt % 4)));
-            if (stages_v) {
-                const char *vr = row_at(a.v_cache, id_k, pos) + (uint32_t)((tid / DW % 4) * 4 * D + 4 * (tid % DW));
 #pragma unroll
-                for (int r = 0; r < 4; r++) vreg[r] = *reinterpret_cast<const uint32_t *>(vr + r * D);
+        for (int i = 0; i < NU; i++) {
+            const int u = stager + STAGERS * i;
+            if constexpr (PAGE16) {
+                const int pos = first16(key0, i);
+                if (stages_k) kreg[i] = *reinterpret_cast<const u32x4 *>(row_at(a.k_cache, id_k[i], pos) + (uint32_t)((u / (D / 16) % 16) * D + 16 * (u % (D / 16))));
+                if (stages_v) {
+                    const char *vr = row_at(a.v_cache, id_k[i], pos) + (uint32_t)((u / DW % 4) * 4 * D + 4 * (u % DW));
+#pragma unroll
+                    for (int r = 0; r < 4; r++) vreg[i][r] = *reinterpret_cast<const uint32_t *>(vr + r * D);
+                }
+            } else {
+                if (stages_k) kreg[i] = *reinterpret_cast<const u32x4 *>(row_at(a.k_cache, id_k[i], min(key0 + u / (D / 16), key_end - 1)) + 16 * (u % (D / 16)));
+                if (stages_v)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        vreg[i][r] = *reinterpret_cast<const uint32_t *>(row_at(a.v_cache, id_v[i][r], min(key0 + 4 * (u / DW) + r, key_end - 1)) + 4 * (u % DW));
             }
-        } else {
-            if (stages_k) kreg = *reinterpret_cast<const u32x4 *>(row_at(a.k_cache, id_k, min(key0 + kt / 4, key_end - 1)) + 16 * (kt % 4));
-            if (stages_v)
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-                    vreg[r] = *reinterpret_cast<const uint32_t *>(row_at(a.v_cache, id_v[r], min(key0 + 4 * (tid / DW) + r, key_end - 1)) + 4 * (tid % DW));
         }
     };
     auto on_diag = [&](int key0) { return min(key0 + BN, key_end) - 1 > tile_first; };   // some column does not see some key of the tile
@@ -661,52 +672,56 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn64_kernel(ChunkArgs
         int nf = 0;
         unsigned char *k_lds = smem + buf * kBufBytes;
         _Float16 *vt_lds = reinterpret_cast<_Float16 *>(k_lds + BN * KP);
-        if (stages_k) {
-            const int key = kt / 4, c16 = kt % 4;
-            if constexpr (BF8) {
-                *reinterpret_cast<u32x4 *>(k_lds + key * KP + 16 * c16) = kreg;
-            } else {
-                half8_t *kd = reinterpret_cast<half8_t *>(k_lds + key * KP + 32 * c16);
-                kd[0] = chunk_dec8<MODE>(kreg.x, kreg.y);
-                kd[1] = chunk_dec8<MODE>(kreg.z, kreg.w);
+#pragma unroll
+        for (int i = 0; i < NU; i++) {
+            const int u = stager + STAGERS * i;
+            if (stages_k) {
+                const int key = u / (D / 16), c16 = u % (D / 16);
+                if constexpr (BF8) {
+                    *reinterpret_cast<u32x4 *>(k_lds + key * KP + 16 * c16) = kreg[i];
+                } else {
+                    half8_t *kd = reinterpret_cast<half8_t *>(k_lds + key * KP + 32 * c16);
+                    kd[0] = chunk_dec8<MODE>(kreg[i].x, kreg[i].y);
+                    kd[1] = chunk_dec8<MODE>(kreg[i].z, kreg[i].w);
+                }
             }
-        }
-        if (stages_v) {
-            const int ddw = tid % DW, kg = tid / DW;
-            const int q4 = kg & 3, pos = 16 * (kg >> 2) + 8 * (q4 & 1) + 4 * (q4 >> 1);
-            const bool whole = key0 + BN <= key_end;
-            if (!whole)
+            if (stages_v) {
+                const int ddw = u % DW, kg = u / DW;
+                const int q4 = kg & 3, pos = 16 * (kg >> 2) + 8 * (q4 & 1) + 4 * (q4 >> 1);
+                uint32_t (&w)[4] = vreg[i];
+                if (key0 + BN > key_end)
 #pragma unroll
-                for (int r = 0; r < 4; r++) vreg[r] = key0 + 4 * kg + r < key_end ? vreg[r] : 0u;
-            uint32_t lo2[4], hi2[4];             // halfs (key 0, key 1) and (key 2, key 3) of dim 4 ddw + c
-            if constexpr (BF8) {
-                if (on_diag(key0)) {
+                    for (int r = 0; r < 4; r++) w[r] = key0 + 4 * kg + r < key_end ? w[r] : 0u;
+                uint32_t lo2[4], hi2[4];         // halfs (key 0, key 1) and (key 2, key 3) of dim 4 ddw + c
+                if constexpr (BF8) {
+                    if (on_diag(key0)) {
 #pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const uint32_t m = chunk_nonfinite(vreg[r]);
-                        vreg[r] &= ~m;
-                        nf |= m != 0;
+                        for (int r = 0; r < 4; r++) {
+                            const uint32_t m = chunk_nonfinite(w[r]);
+                            w[r] &= ~m;
+                            nf |= m != 0;
+                        }
                     }
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        const uint32_t sel = 0x000c000cu | ((uint32_t)c << 8) | ((uint32_t)(4 + c) << 24);
+                        lo2[c] = perm(w[1], w[0], sel);
+                        hi2[c] = perm(w[3], w[2], sel);
+                    }
+                } else {
+                    uint32_t p01[4], p23[4];
+#pragma unroll
+                    for (int r = 0; r < 4; r++) dec_word<MODE>(w[r], p01[r], p23[r]);
+                    lo2[0] = perm(p01[1], p01[0], 0x05040100u); hi2[0] = perm(p01[3], p01[2], 0x05040100u);
+                    lo2[1] = perm(p01[1], p01[0], 0x07060302u); hi2[1] = perm(p01[3], p01[2], 0x07060302u);
+                    lo2[2] = perm(p23[1], p23[0], 0x05040100u); hi2[2] = perm(p23[3], p23[2], 0x05040100u);
+                    lo2[3] = perm(p23[1], p23[0], 0x07060302u); hi2[3] = perm(p23[3], p23[2], 0x07060302u);
                 }
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    const uint32_t sel = 0x000c000cu | ((uint32_t)c << 8) | ((uint32_t)(4 + c) << 24);
-                    lo2[c] = perm(vreg[1], vreg[0], sel);
-                    hi2[c] = perm(vreg[3], vreg[2], sel);
+                    const int row = 4 * ddw + c;
+                    *reinterpret_cast<u32x2 *>(vt_lds + row * VS + (((pos >> 3) ^ swz(row)) << 3) + (pos & 4)) = u32x2{lo2[c], hi2[c]};
                 }
-            } else {
-                uint32_t p01[4], p23[4];
-#pragma unroll
-                for (int r = 0; r < 4; r++) dec_word<MODE>(vreg[r], p01[r], p23[r]);
-                lo2[0] = perm(p01[1], p01[0], 0x05040100u); hi2[0] = perm(p01[3], p01[2], 0x05040100u);
-                lo2[1] = perm(p01[1], p01[0], 0x07060302u); hi2[1] = perm(p01[3], p01[2], 0x07060302u);
-                lo2[2] = perm(p23[1], p23[0], 0x05040100u); hi2[2] = perm(p23[3], p23[2], 0x05040100u);
-                lo2[3] = perm(p23[1], p23[0], 0x07060302u); hi2[3] = perm(p23[3], p23[2], 0x07060302u);
-            }
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const int row = 4 * ddw + c;
-                *reinterpret_cast<u32x2 *>(vt_lds + row * VS + (((pos >> 3) ^ swz(row)) << 3) + (pos & 4)) = u32x2{lo2[c], hi2[c]};
             }
         }
         return nf;
@@ -740,36 +755,37 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn64_kernel(ChunkArgs
         }
         const bool masked = key0 + BN - 1 > wave_first;           // wave-uniform: some column does not see some key
         if (wave_has && key0 <= wave_last) {
-            half8_t vf[4][2];   // [16-key step][32-dim block]
+            auto v_frag = [&](int g, int d) {   // 16-key step, 32-dim block
+                const int row = 32 * d + n;
+                return *reinterpret_cast<const half8_t *>(vt_lds + row * VS + (((2 * g + h) ^ swz(row)) << 3));
+            };
+            half8_t vf[4][D == 64 ? 2 : 1];     // d = 64: all of them, requested ahead of the scores
+            if constexpr (D == 64)
 #pragma unroll
-            for (int g = 0; g < 4; g++)
+                for (int g = 0; g < 4; g++)
 #pragma unroll
-                for (int d = 0; d < 2; d++) {
-                    const int row = 32 * d + n;
-                    vf[g][d] = *reinterpret_cast<const half8_t *>(vt_lds + row * VS + (((2 * g + h) ^ swz(row)) << 3));
-                }
+                    for (int d = 0; d < 2; d++) vf[g][d] = v_frag(g, d);
             float16_t sc[CB][2];
             const float16_t zero16 = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int c = 0; c < 2; c++) {
-                if constexpr (BF8) {
-                    const u32x4 *src = reinterpret_cast<const u32x4 *>(k_lds + (32 * c + n) * KP + 32 * h);
-                    const u32x4 w0 = src[0], w1 = src[1];
-                    const int8p_t kf = {(int)w0.x, (int)w0.y, (int)w0.z, (int)w0.w, (int)w1.x, (int)w1.y, (int)w1.z, (int)w1.w};
+            for (int c = 0; c < 2; c++)
 #pragma unroll
-                    for (int b = 0; b < CB; b++)   // both operands in the BF8 (E5M2) format, no block scales
-                        sc[b][c] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf, qf[b], zero16, 1, 1, 0, 0, 0, 0);
-                } else {
-                    half8_t k16[4];
+                for (int st = 0; st < STEPS; st++) {
+                    if constexpr (BF8) {
+                        const u32x4 *src = reinterpret_cast<const u32x4 *>(k_lds + (32 * c + n) * KP + 64 * st + 32 * h);
+                        const u32x4 w0 = src[0], w1 = src[1];
+                        const int8p_t kf = {(int)w0.x, (int)w0.y, (int)w0.z, (int)w0.w, (int)w1.x, (int)w1.y, (int)w1.z, (int)w1.w};
 #pragma unroll
-                    for (int st = 0; st < 4; st++) k16[st] = *reinterpret_cast<const half8_t *>(k_lds + (32 * c + n) * KP + 32 * st + 16 * h);
+                        for (int b = 0; b < CB; b++)   // both operands in the BF8 (E5M2) format, no block scales
+                            sc[b][c] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf, qf[b][st], st == 0 ? zero16 : sc[b][c], 1, 1, 0, 0, 0, 0);
+                    } else {
+                        const half8_t k16 = *reinterpret_cast<const half8_t *>(k_lds + (32 * c + n) * KP + 32 * st + 16 * h);
 #pragma unroll
-                    for (int b = 0; b < CB; b++)
-#pragma unroll
-                        for (int st = 0; st < 4; st++)
-                            sc[b][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k16[st], qh16[b][st], st == 0 ? zero16 : sc[b][c], 0, 0, 0);
+                        for (int b = 0; b < CB; b++)
+                            sc[b][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k16, qh16[b][st], st == 0 ? zero16 : sc[b][c], 0, 0, 0);
+                    }
                 }
-            }
+            half8_t pb[CB][4];
 #pragma unroll
             for (int b = 0; b < CB; b++) {
                 if (masked) {
@@ -783,7 +799,6 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn64_kernel(ChunkArgs
                 }
                 // P against the column's current reference point; the lane's share of the sum tells whether that was safe
                 // (see kGuard); if not, the reference is raised to the true maximum and P computed again
-                half8_t pb[4];
                 auto exp_block = [&](const float mc) {
                     float sum = 0.f;
 #pragma unroll
@@ -796,7 +811,7 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn64_kernel(ChunkArgs
                             pw[i] = as_u32(__builtin_convertvector(float2p_t{e0, e1}, half2_t));
                             sum = dot2(pw[i], 0x3c003c00u, sum);  // the sum takes the rounded values that multiply V
                         }
-                        pb[g] = __builtin_bit_cast(half8_t, u32x4{pw[0], pw[1], pw[2], pw[3]});
+                        pb[b][g] = __builtin_bit_cast(half8_t, u32x4{pw[0], pw[1], pw[2], pw[3]});
                     }
                     return sum;
                 };
@@ -814,20 +829,30 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn64_kernel(ChunkArgs
                     mc_run[b] = m_new * a.scale_log2e;
                     l_run[b] *= alpha;
 #pragma unroll
-                    for (int d = 0; d < 2; d++) o[b][d] *= alpha;
+                    for (int d = 0; d < DB; d++) o[b][d] *= alpha;
                     sum = exp_block(m_new == -INFINITY ? 0.f : mc_run[b]);
                 }
                 l_run[b] += sum;
+                if constexpr (D == 64)
 #pragma unroll
-                for (int g = 0; g < 4; g++)
+                    for (int g = 0; g < 4; g++)
 #pragma unroll
-                    for (int d = 0; d < 2; d++) o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[g][d], pb[g], o[b][d], 0, 0, 0);
+                        for (int d = 0; d < 2; d++) o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[g][d], pb[b][g], o[b][d], 0, 0, 0);
             }
+            if constexpr (D > 64)
+#pragma unroll
+                for (int d = 0; d < DB; d++)
+#pragma unroll
+                    for (int g = 0; g < 4; g++) {
+                        const half8_t v1 = v_frag(g, d);
+#pragma unroll
+                        for (int b = 0; b < CB; b++) o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, pb[b][g], o[b][d], 0, 0, 0);
+                    }
             if (BF8 && nf) {   // rare: what the staged zeros stand for, added for the columns that see the key
                 for (int key = key0; key < min(key0 + BN, key_end); key++) {
                     const uint32_t *vr = reinterpret_cast<const uint32_t *>(row_at(a.v_cache, bt[chunk_block_of(a, key)], key)) + h;
 #pragma unroll
-                    for (int d = 0; d < 2; d++)
+                    for (int d = 0; d < DB; d++)
 #pragma unroll
                         for (int g = 0; g < 4; g++) {             // dims 32 d + 8 g + 4 h + {0..3}
                             const uint32_t w = vr[8 * d + 2 * g], m = chunk_nonfinite(w);
@@ -865,7 +890,7 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn64_kernel(ChunkArgs
         const int64_t items = (int64_t)a.total_rows * a.n_q_heads, at = zr * items + item[b];
         const float inv = l == 0.f ? 0.f : 1.0f / l;              // no visible key: a zero result
 #pragma unroll
-        for (int d = 0; d < 2; d++)
+        for (int d = 0; d < DB; d++)
 #pragma unroll
             for (int g = 0; g < 4; g++) {
                 const float4_t x = {o[b][d][4 * g], o[b][d][4 * g + 1], o[b][d][4 * g + 2], o[b][d][4 * g + 3]};
@@ -1459,11 +1484,15 @@ struct ChunkPlan {
 // Steps in the ring of a wave of the narrow kernel (0: the rows go through registers).
 static constexpr int ring_steps(int d, int nb) { return d == 64 ? 4 : (d == 128 ? (nb == 4 ? 4 : 2) : (d == 256 ? 2 : 0)); }
 
-constexpr int kWide64Blocks = 2;   // 32-column blocks of a wave of the d = 64 kernel (256 columns per workgroup)
-
 static int log2_of(int64_t x) { int l = 0; while ((1ll << l) < x) l++; return l; }
 
-static int wide_columns(int64_t d) { return d == 64 ? 256 : (d == 512 ? 64 : 128); }
+// Workgroup of the LDS kernels per head dim: columns, waves, keys per tile, and waves per SIMD that the registers are for.
+struct WideShape { int columns, waves, keys, occ; };
+constexpr int kMost32 = 128;             // largest head dim on the 32x32 instructions
+static constexpr WideShape wide_shape(int64_t d) {
+    return d == 64 ? WideShape{256, 4, 64, 2} : (d == 128 ? WideShape{128, 4, 64, 2} : (d == 256 ? WideShape{128, 8, 64, 1} : WideShape{64, 4, 32, 1}));
+}
+static int wide_columns(int64_t d) { return wide_shape(d).columns; }
 static int narrow_most_blocks(int64_t d) { return d <= 128 ? 4 : (d == 256 ? 2 : 1); }
 
 static int64_t chunk_slots(int64_t total_rows, int64_t n_seq, int64_t group, int qt) { return total_rows * group / qt + n_seq; }
@@ -1517,23 +1546,21 @@ static int64_t chunk_narrow_scratch(const ChunkPlan &p) { return p.z_narrow > 1 
 
 template <int D, int MODE, bool PAGE16, bool ZS>
 static int launch_chunk_wide(const ChunkArgs &a, bool fill, hipStream_t s) {
-    constexpr int QB = D == 128 ? 2 : 1, BN = D == 512 ? 32 : 64, OCC = D <= 128 ? 2 : 1, WAVES = D == 256 ? 8 : 4;
-    constexpr int QT = D == 64 ? 256 : 16 * QB * WAVES;
-    constexpr int KS = MODE == FEATHER_E5M2 ? (D + 16) / 2 : D + 8;
-    constexpr size_t lds = (size_t)(BN * KS + D * BN) * 2 * 2;
+    constexpr WideShape w = wide_shape(D);
+    constexpr int KS = MODE == FEATHER_E5M2 ? (D + 16) / 2 : D + 8;   // K row pitch in fp16 units, as in the kernels
+    constexpr size_t lds = (size_t)(w.keys * KS + D * w.keys) * 2 * 2;
     const char *me = "feather_paged_chunk_attn_fp8";
-    const int64_t slots = chunk_slots(a.total_rows, a.n_seq, a.group, QT);
+    const int64_t slots = chunk_slots(a.total_rows, a.n_seq, a.group, w.columns);
     const int64_t blocks = slots * a.n_kv_heads * a.z_wide;
     FEATHER_CHECK(blocks + kChunkFillGroups < (1ll << 31), FEATHER_ESHAPE, "%s: grid too large", me);
     auto kern = [] {
-        if constexpr (D == 64) return chunk_attn64_kernel<MODE, kWide64Blocks, 256 / (32 * kWide64Blocks), 2, PAGE16, ZS>;
-        else return chunk_attn_kernel<D, MODE, QB, BN, OCC, WAVES, PAGE16, ZS>;
+        if constexpr (D <= kMost32) return chunk_attn32_kernel<D, MODE, w.columns / (32 * w.waves), w.waves, w.occ, PAGE16, ZS>;
+        else return chunk_attn_kernel<D, MODE, w.columns / (16 * w.waves), w.keys, w.occ, w.waves, PAGE16, ZS>;
     }();
-    constexpr int threads = D == 64 ? 64 * (256 / (32 * kWide64Blocks)) : 64 * WAVES;
     static unsigned long long lds_raised = 0;
     hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(kern), lds, lds_raised);
     FEATHER_CHECK(e == hipSuccess, FEATHER_ELAUNCH, "%s: cannot raise LDS limit: %s", me, hipGetErrorString(e));
-    hipLaunchKernelGGL(kern, dim3((unsigned)(blocks + (fill ? kChunkFillGroups : 0))), dim3(threads), lds, s, a, (int)slots);
+    hipLaunchKernelGGL(kern, dim3((unsigned)(blocks + (fill ? kChunkFillGroups : 0))), dim3(64 * w.waves), lds, s, a, (int)slots);
     return check_launch(me);
 }
 
@@ -1574,7 +1601,7 @@ static int launch_chunk(const ChunkArgs &a, const ChunkPlan &p, hipStream_t s) {
     while (!p.wide && (4 << zl) < a.z_narrow && (DW << zl) < 256) zl++;
     const int64_t per_group = (256 / DW) >> zl, items = (int64_t)a.total_rows * a.n_q_heads;
     hipLaunchKernelGGL((chunk_merge_kernel<D, MODE>), dim3((unsigned)((items + per_group - 1) / per_group)), dim3(256), 0, s, a,
-                       log2_of(wide_columns(D)), D == 512 ? 32 : 64, log2_of(16 * p.nb), zl);
+                       log2_of(wide_columns(D)), wide_shape(D).keys, log2_of(16 * p.nb), zl);
     return check_launch("feather_paged_chunk_attn_fp8 (merge of the key ranges)");
 }
 
