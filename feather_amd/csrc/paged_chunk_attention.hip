@@ -184,8 +184,8 @@ constexpr int kAnyColumns = 1 << 30;   // more columns than a call can have
 // of BN keys are fetched packed through the block table into registers two tiles ahead (their block ids three tiles
 // ahead: a table entry is never waited for), decoded into the other LDS buffer one tile ahead, and read by all waves.
 // ALIGN4: block_size % 4 == 0, so four keys from a multiple of four on share a block (one table lookup).
-template <int D, int MODE, int QB, int BN, int OCC, int WAVES, bool ALIGN4, bool ZS>
-__global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn_kernel(ChunkArgs a, int n_slots) {
+template <int D, int MODE, int QB, int BN, int WAVES, bool ALIGN4, bool ZS>
+__device__ __forceinline__ void chunk_attn_body(const ChunkArgs &a, int n_slots, int bid) {
     constexpr int DW = D / 4;
     constexpr bool BF8 = MODE == FEATHER_E5M2;
     constexpr int KS = BF8 ? (D + 16) / 2 : D + 8;   // K row pitch in LDS, in fp16 units (bf8: D + 16 bytes)
@@ -202,12 +202,6 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn_kernel(ChunkArgs a
     _Float16 *const lds = reinterpret_cast<_Float16 *>(smem);
     auto swz = [](int row) { return (row ^ (row >> 2)) & (CH - 1); };
 
-    const int work = n_slots * a.n_kv_heads * (ZS ? a.z_wide : 1);
-    int bid = blockIdx.x;
-    if (bid >= work) {
-        chunk_fill_outside<D>(a, bid - work, gridDim.x - work, kThreads);
-        return;
-    }
     // Launch order goes round the XCDs (own L2 each): with the KV head fastest an XCD keeps to few heads, and with the tiles
     // slowest the longest tiles of all heads start first on all of them.
     const int kvh = bid % a.n_kv_heads;
@@ -525,8 +519,8 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn_kernel(ChunkArgs a
 // PAGE16 (block_size % 16 == 0): the 16 keys that a wave stages share a block, whose address is then scalar.
 typedef int int8p_t __attribute__((ext_vector_type(8)));
 
-template <int D, int MODE, int CB, int WAVES, int OCC, bool PAGE16, bool ZS>
-__global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn32_kernel(ChunkArgs a, int n_slots) {
+template <int D, int MODE, int CB, int WAVES, bool PAGE16, bool ZS>
+__device__ __forceinline__ void chunk_attn32_body(const ChunkArgs &a, int n_slots, int bid) {
     constexpr bool BF8 = MODE == FEATHER_E5M2;
     constexpr int DW = D / 4, BN = 64, DB = D / 32, STEPS = BF8 ? D / 64 : D / 16;   // 32-dim blocks; matrix steps of a score block
     constexpr int KP = (BF8 ? D : 2 * D) + 16;   // K row pitch in LDS, bytes
@@ -540,12 +534,6 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void chunk_attn32_kernel(ChunkArgs
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     auto swz = [](int row) { return ((row >> 1) & 7) ^ ((row >> 4) & 1); };   // 16-byte chunk c of V^T row r lives at chunk c ^ swz(r)
 
-    const int work = n_slots * a.n_kv_heads * (ZS ? a.z_wide : 1);
-    int bid = blockIdx.x;
-    if (bid >= work) {
-        chunk_fill_outside<D>(a, bid - work, gridDim.x - work, kThreads);
-        return;
-    }
     // Launch order goes round the XCDs (own L2 each): with the KV head fastest an XCD keeps to few heads, and with the tiles
     // slowest the longest tiles of all heads start first on all of them.
     const int kvh = bid % a.n_kv_heads;
@@ -962,7 +950,7 @@ __device__ __forceinline__ int64_t narrow_item(const ChunkArgs &a, int64_t item,
 }
 
 template <int D, int MODE, int NB, int RING>
-__global__ __launch_bounds__(256, (D / 64) * NB <= 4 ? 2 : 1) void chunk_narrow_kernel(ChunkArgs a, int fill) {
+__device__ __forceinline__ void chunk_narrow_body(const ChunkArgs &a, int pair, int zr) {
     constexpr int DW = D / 4, RB = D / 64, STEPS = D / 32, QT = 16 * NB, W = 4, STEP = 32;
     constexpr bool BF8 = MODE == FEATHER_E5M2;
     constexpr int NF = RING > 0 ? 1 : (D == 64 ? (NB == 4 ? 2 : 4) : (D == 128 ? 2 : 1));
@@ -971,13 +959,10 @@ __global__ __launch_bounds__(256, (D / 64) * NB <= 4 ? 2 : 1) void chunk_narrow_
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     float4_t *const x_lds = reinterpret_cast<float4_t *>(smem);     // [NB][W][RB * 4][64]
 
-    // Grid (sequence and KV head, key range).  In launch order, which goes round the XCDs, all first ranges come before all
-    // second ones and so on: ranges that do not exist come last.  A sequence has one tile here -- unless the caller's
-    // bound of its rows was wrong, then the workgroup takes its tiles one after the other.
-    const int zr = blockIdx.y;
-    if (fill && zr == 0) chunk_fill_outside<D>(a, blockIdx.x, gridDim.x, 256);
-    if (a.n_seq == 0) return;
-    const int seq_i = (int)(__umulhi(2u * blockIdx.x, a.kv_mul) >> a.kv_shift), kvh = blockIdx.x - seq_i * a.n_kv_heads;
+    // In launch order, which goes round the XCDs, all first ranges come before all second ones and so on: ranges that do
+    // not exist come last.  A sequence has one tile here -- unless the caller's bound of its rows was wrong, then the
+    // workgroup takes its tiles one after the other.
+    const int seq_i = (int)(__umulhi(2u * (uint32_t)pair, a.kv_mul) >> a.kv_shift), kvh = pair - seq_i * a.n_kv_heads;
     ChunkTile t;
     t.seq = seq_i;
     t.row0 = chunk_clamp_row(a.cu_seqlens[seq_i], a.total_rows);
@@ -987,7 +972,7 @@ __global__ __launch_bounds__(256, (D / 64) * NB <= 4 ? 2 : 1) void chunk_narrow_
     int least = kNarrowMinKeys;
     if (a.z_narrow > 1) {
         least = narrow_min_keys(a, QT);
-        if (blockIdx.x + blockIdx.y == 0 && threadIdx.x == 0) *reinterpret_cast<int *>(a.part_narrow + narrow_items(a) * a.z_narrow * (D + 2)) = least;
+        if (pair + zr == 0 && threadIdx.x == 0) *reinterpret_cast<int *>(a.part_narrow + narrow_items(a) * a.z_narrow * (D + 2)) = least;
     }
     if (t.cols > a.col_split) return;                               // a long run of rows: the other kernel's work
 #pragma nounroll
@@ -1362,6 +1347,66 @@ __global__ __launch_bounds__(256, (D / 64) * NB <= 4 ? 2 : 1) void chunk_narrow_
     }
 }
 
+// ---- kernels: the LDS kernel alone, the narrow one alone, or both in one grid ------------------------------------------
+// Workgroup of the LDS kernels per head dim: columns, waves, keys per tile, and waves per SIMD that the registers are for.
+struct WideShape { int columns, waves, keys, occ; };
+constexpr int kMost32 = 128;             // largest head dim on the 32x32 instructions
+static constexpr WideShape wide_shape(int64_t d) {
+    return d == 64 ? WideShape{256, 4, 64, 2} : (d == 128 ? WideShape{128, 4, 64, 2} : (d == 256 ? WideShape{128, 8, 64, 1} : WideShape{64, 4, 32, 1}));
+}
+// Steps in the ring of a wave of the narrow kernel (0: the rows go through registers).
+static constexpr int ring_steps(int d, int nb) { return d == 64 ? 4 : (d == 128 ? (nb == 4 ? 4 : 2) : (d == 256 ? 2 : 0)); }
+
+constexpr int mixed_blocks(int d) { return d <= 256 ? 2 : 1; }   // 16-column blocks of the narrow kernel beside the LDS kernel
+constexpr size_t wide_lds(int d, int mode) {   // two (K, V^T) buffers; K rows of d bytes (E5M2) or halfs, 16 bytes more each
+    const WideShape w = wide_shape(d);
+    return (size_t)(w.keys * (mode == FEATHER_E5M2 ? d + 16 : 2 * d + 16) + 2 * d * w.keys) * 2;
+}
+constexpr size_t narrow_lds(int d, int nb, int ring) {   // the rings, or the exchange at the end
+    const size_t join = (size_t)nb * d * 256, rings = (size_t)4 * ring * 64 * d;
+    return join > rings ? join : rings;
+}
+
+template <int D, int MODE, bool PAGE16, bool ZS>
+__device__ __forceinline__ void chunk_wide_body(const ChunkArgs &a, int n_slots, int bid) {
+    constexpr WideShape w = wide_shape(D);
+    if constexpr (D <= kMost32) chunk_attn32_body<D, MODE, w.columns / (32 * w.waves), w.waves, PAGE16, ZS>(a, n_slots, bid);
+    else chunk_attn_body<D, MODE, w.columns / (16 * w.waves), w.keys, w.waves, PAGE16, ZS>(a, n_slots, bid);
+}
+
+template <int D, int MODE, bool PAGE16, bool ZS>
+__global__ __launch_bounds__(64 * wide_shape(D).waves, wide_shape(D).occ) void chunk_wide_kernel(ChunkArgs a, int n_slots) {
+    const int work = n_slots * a.n_kv_heads * (ZS ? a.z_wide : 1), bid = blockIdx.x;
+    if (bid < work) chunk_wide_body<D, MODE, PAGE16, ZS>(a, n_slots, bid);
+    else chunk_fill_outside<D>(a, bid - work, gridDim.x - work, 64 * wide_shape(D).waves);
+}
+
+template <int D, int MODE, int NB, int RING>
+__global__ __launch_bounds__(256, (D / 64) * NB <= 4 ? 2 : 1) void chunk_narrow_kernel(ChunkArgs a, int fill) {
+    if (fill && blockIdx.y == 0) chunk_fill_outside<D>(a, blockIdx.x, gridDim.x, 256);
+    if (a.n_seq > 0) chunk_narrow_body<D, MODE, NB, RING>(a, blockIdx.x, blockIdx.y);
+}
+
+// A batch of long and short runs of rows: the tiles first, whose matrix work then shares the CUs with the streaming of the
+// short ones' caches (one after the other they leave the memory and the matrix cores idle in turn).
+template <int D, int MODE, bool PAGE16, bool ZS>
+__global__ __launch_bounds__(256, wide_shape(D).occ) void chunk_mixed_kernel(ChunkArgs a, int n_slots) {
+    constexpr int NB = mixed_blocks(D);
+    int bid = blockIdx.x;
+    const int wide = n_slots * a.n_kv_heads * (ZS ? a.z_wide : 1), pairs = a.n_seq * a.n_kv_heads, narrow = pairs * a.z_narrow;
+    if (bid < wide) {
+        chunk_wide_body<D, MODE, PAGE16, ZS>(a, n_slots, bid);
+        return;
+    }
+    bid -= wide;
+    if (bid < narrow) {
+        const int zr = bid / pairs;
+        chunk_narrow_body<D, MODE, NB, PAGE16 ? ring_steps(D, NB) : 0>(a, bid - zr * pairs, zr);
+    } else {
+        chunk_fill_outside<D>(a, bid - narrow, gridDim.x - wide - narrow, 256);
+    }
+}
+
 // Adds the key ranges of a column in range order.  A workgroup holds 256 / (DW * zl) items (row, head); an item's dims
 // lie along DW threads, and zl of these rows of threads take the item's ranges in turn and are joined through LDS, so
 // that few items of many ranges are not one long chain of loads.  Rows of no sequence are zeroed here (fill) or left
@@ -1481,17 +1526,8 @@ struct ChunkPlan {
     int64_t wide_bytes, narrow_bytes;   // of the workspace, per range
 };
 
-// Steps in the ring of a wave of the narrow kernel (0: the rows go through registers).
-static constexpr int ring_steps(int d, int nb) { return d == 64 ? 4 : (d == 128 ? (nb == 4 ? 4 : 2) : (d == 256 ? 2 : 0)); }
-
 static int log2_of(int64_t x) { int l = 0; while ((1ll << l) < x) l++; return l; }
 
-// Workgroup of the LDS kernels per head dim: columns, waves, keys per tile, and waves per SIMD that the registers are for.
-struct WideShape { int columns, waves, keys, occ; };
-constexpr int kMost32 = 128;             // largest head dim on the 32x32 instructions
-static constexpr WideShape wide_shape(int64_t d) {
-    return d == 64 ? WideShape{256, 4, 64, 2} : (d == 128 ? WideShape{128, 4, 64, 2} : (d == 256 ? WideShape{128, 8, 64, 1} : WideShape{64, 4, 32, 1}));
-}
 static int wide_columns(int64_t d) { return wide_shape(d).columns; }
 static int narrow_most_blocks(int64_t d) { return d <= 128 ? 4 : (d == 256 ? 2 : 1); }
 
@@ -1519,7 +1555,7 @@ static ChunkPlan chunk_plan(int64_t n_seq, int64_t total_rows, int64_t n_q_heads
         p.nb = cols <= 16 ? 1 : (cols <= 32 ? 2 : 4);
     } else {
         p.wide = true;
-        p.nb = narrow_most_blocks(d) >= 2 ? 2 : 1;
+        p.nb = mixed_blocks((int)d);
         // with n_seq - 1 sequences of the longest length, can the last one be short?  (If the hint is wrong the LDS kernel
         // takes the short ones too.)
         const int64_t least = total_rows - (n_seq - 1) * rows_most;
@@ -1544,51 +1580,53 @@ static ChunkPlan chunk_plan(int64_t n_seq, int64_t total_rows, int64_t n_q_heads
 static int64_t chunk_wide_scratch(const ChunkPlan &p) { return p.z_wide > 1 ? (p.z_wide * p.wide_bytes + 15) / 16 * 16 : 0; }
 static int64_t chunk_narrow_scratch(const ChunkPlan &p) { return p.z_narrow > 1 ? p.z_narrow * p.narrow_bytes + 16 : 0; }
 
-template <int D, int MODE, bool PAGE16, bool ZS>
-static int launch_chunk_wide(const ChunkArgs &a, bool fill, hipStream_t s) {
-    constexpr WideShape w = wide_shape(D);
-    constexpr int KS = MODE == FEATHER_E5M2 ? (D + 16) / 2 : D + 8;   // K row pitch in fp16 units, as in the kernels
-    constexpr size_t lds = (size_t)(w.keys * KS + D * w.keys) * 2 * 2;
+template <class Kernel>
+static int launch_chunk_kernel(Kernel kern, dim3 grid, int threads, size_t lds, hipStream_t s, const ChunkArgs &a, int arg, unsigned long long &lds_raised) {
     const char *me = "feather_paged_chunk_attn_fp8";
-    const int64_t slots = chunk_slots(a.total_rows, a.n_seq, a.group, w.columns);
-    const int64_t blocks = slots * a.n_kv_heads * a.z_wide;
-    FEATHER_CHECK(blocks + kChunkFillGroups < (1ll << 31), FEATHER_ESHAPE, "%s: grid too large", me);
-    auto kern = [] {
-        if constexpr (D <= kMost32) return chunk_attn32_kernel<D, MODE, w.columns / (32 * w.waves), w.waves, w.occ, PAGE16, ZS>;
-        else return chunk_attn_kernel<D, MODE, w.columns / (16 * w.waves), w.keys, w.occ, w.waves, PAGE16, ZS>;
-    }();
-    static unsigned long long lds_raised = 0;
-    hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(kern), lds, lds_raised);
+    hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(kern), lds + 4096, lds_raised);   // (and the kernels' static arrays)
     FEATHER_CHECK(e == hipSuccess, FEATHER_ELAUNCH, "%s: cannot raise LDS limit: %s", me, hipGetErrorString(e));
-    hipLaunchKernelGGL(kern, dim3((unsigned)(blocks + (fill ? kChunkFillGroups : 0))), dim3(64 * w.waves), lds, s, a, (int)slots);
+    hipLaunchKernelGGL(kern, grid, dim3(threads), lds, s, a, arg);
     return check_launch(me);
 }
 
 template <int D, int MODE, int NB, int RING>
 static int launch_chunk_narrow(const ChunkArgs &a, bool fill, hipStream_t s) {
-    constexpr size_t join = (size_t)NB * 4 * (D / 64) * 4 * 64 * 16, rings = (size_t)4 * RING * 64 * D, lds = join > rings ? join : rings;
-    const char *me = "feather_paged_chunk_attn_fp8";
     const int64_t pairs = a.n_seq > 0 ? (int64_t)a.n_seq * a.n_kv_heads : kChunkFillGroups;
-    FEATHER_CHECK(pairs * a.z_narrow < (1ll << 31), FEATHER_ESHAPE, "%s: grid too large", me);
-    auto kern = chunk_narrow_kernel<D, MODE, NB, RING>;
+    FEATHER_CHECK(pairs * a.z_narrow < (1ll << 31), FEATHER_ESHAPE, "feather_paged_chunk_attn_fp8: grid too large");
     static unsigned long long lds_raised = 0;
-    hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(kern), lds + 4096, lds_raised);
-    FEATHER_CHECK(e == hipSuccess, FEATHER_ELAUNCH, "%s: cannot raise LDS limit: %s", me, hipGetErrorString(e));
-    hipLaunchKernelGGL(kern, dim3((unsigned)pairs, (unsigned)a.z_narrow), dim3(256), lds, s, a, fill ? 1 : 0);
-    return check_launch(me);
+    return launch_chunk_kernel(chunk_narrow_kernel<D, MODE, NB, RING>, dim3((unsigned)pairs, (unsigned)a.z_narrow), 256, narrow_lds(D, NB, RING), s, a,
+                               fill ? 1 : 0, lds_raised);
+}
+
+template <int D, int MODE, bool PAGE16, bool ZS>
+static int launch_chunk_wide(const ChunkArgs &a, bool narrow, bool fill, hipStream_t s) {
+    constexpr WideShape w = wide_shape(D);
+    constexpr int NB = mixed_blocks(D), RING = PAGE16 ? ring_steps(D, NB) : 0;
+    constexpr bool kOneGrid = w.waves == 4;            // both kernels' workgroups have four waves
+    const int64_t slots = chunk_slots(a.total_rows, a.n_seq, a.group, w.columns);
+    const int64_t wide = slots * a.n_kv_heads * a.z_wide, more = narrow && kOneGrid ? (int64_t)a.n_seq * a.n_kv_heads * a.z_narrow : 0;
+    FEATHER_CHECK(wide + more + kChunkFillGroups < (1ll << 31), FEATHER_ESHAPE, "feather_paged_chunk_attn_fp8: grid too large");
+    const dim3 grid((unsigned)(wide + more + (fill ? kChunkFillGroups : 0)));
+    if constexpr (kOneGrid)
+        if (narrow) {
+            constexpr size_t lds = wide_lds(D, MODE) > narrow_lds(D, NB, RING) ? wide_lds(D, MODE) : narrow_lds(D, NB, RING);
+            static unsigned long long lds_raised = 0;
+            return launch_chunk_kernel(chunk_mixed_kernel<D, MODE, PAGE16, ZS>, grid, 256, lds, s, a, (int)slots, lds_raised);
+        }
+    static unsigned long long lds_raised = 0;
+    const int rc = launch_chunk_kernel(chunk_wide_kernel<D, MODE, PAGE16, ZS>, grid, 64 * w.waves, wide_lds(D, MODE), s, a, (int)slots, lds_raised);
+    if (rc != FEATHER_OK || !narrow) return rc;
+    return launch_chunk_narrow<D, MODE, NB, RING>(a, false, s);
 }
 
 template <int D, int MODE, bool PAGE16>
 static int launch_chunk(const ChunkArgs &a, const ChunkPlan &p, hipStream_t s) {
     const bool merge = a.z_wide > 1 || a.z_narrow > 1;
-    bool fill = a.fill && !merge;                            // rows outside every sequence: the merge's work, or the first kernel's
+    const bool fill = a.fill && !merge;                      // rows outside every sequence: the merge's work, or the first kernel's
     int rc = FEATHER_OK;
     if (p.wide) {
-        rc = a.z_wide > 1 ? launch_chunk_wide<D, MODE, PAGE16, true>(a, fill, s)
-                          : launch_chunk_wide<D, MODE, PAGE16, false>(a, fill, s);
-        fill = false;
-    }
-    if (rc == FEATHER_OK && p.narrow) {
+        rc = a.z_wide > 1 ? launch_chunk_wide<D, MODE, PAGE16, true>(a, p.narrow, fill, s) : launch_chunk_wide<D, MODE, PAGE16, false>(a, p.narrow, fill, s);
+    } else {
         if (p.nb == 1) rc = launch_chunk_narrow<D, MODE, 1, PAGE16 ? ring_steps(D, 1) : 0>(a, fill, s);
         if constexpr (D <= 256)
             if (p.nb == 2) rc = launch_chunk_narrow<D, MODE, 2, PAGE16 ? ring_steps(D, 2) : 0>(a, fill, s);
