@@ -24,8 +24,6 @@ namespace feather {
 
 typedef float float2p_t __attribute__((ext_vector_type(2)));
 
-enum ChunkOut { kChunkF32 = 0, kChunkF16 = 1, kChunkPacked = 2 };
-
 struct ChunkArgs {
     const uint32_t *q, *k_cache, *v_cache;
     const int32_t *block_tables, *cu_seqlens, *ctx_lens;
@@ -128,9 +126,9 @@ __device__ __forceinline__ uint32_t chunk_block_of(const ChunkArgs &a, int pos) 
 // four consecutive dims of one (row, head), starting at dim 4 * w4
 template <int D, int MODE>
 __device__ __forceinline__ void chunk_store(const ChunkArgs &a, int64_t item, int w4, float4_t x) {
-    if (a.out_kind == kChunkF32) {
+    if (a.out_kind == FEATHER_CHUNK_OUT_F32) {
         *reinterpret_cast<float4_t *>(static_cast<float *>(a.out) + item * D + 4 * w4) = x;
-    } else if (a.out_kind == kChunkF16) {
+    } else if (a.out_kind == FEATHER_CHUNK_OUT_F16) {
         const half4_t h = {(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
         *reinterpret_cast<half4_t *>(static_cast<_Float16 *>(a.out) + item * D + 4 * w4) = h;
     } else {
@@ -144,7 +142,7 @@ __device__ __forceinline__ void chunk_fill_outside(const ChunkArgs &a, int part,
     const int first = a.n_seq > 0 ? chunk_clamp_row(a.cu_seqlens[0], a.total_rows) : a.total_rows;
     const int last = a.n_seq > 0 ? max(chunk_clamp_row(a.cu_seqlens[a.n_seq], a.total_rows), first) : a.total_rows;
     const int64_t unit = (int64_t)a.n_q_heads * D / 4;                     // packed words of a row
-    const int words = a.out_kind == kChunkF32 ? 4 : (a.out_kind == kChunkF16 ? 2 : 1);
+    const int words = a.out_kind == FEATHER_CHUNK_OUT_F32 ? 4 : (a.out_kind == FEATHER_CHUNK_OUT_F16 ? 2 : 1);
     uint32_t *out = static_cast<uint32_t *>(a.out);
     for (int64_t i = (int64_t)part * threads + threadIdx.x; i < (first + (int64_t)(a.total_rows - last)) * unit * words;
          i += (int64_t)parts * threads) {
@@ -185,16 +183,15 @@ constexpr int kAnyColumns = 1 << 30;   // more columns than a call can have
 // ahead: a table entry is never waited for), decoded into the other LDS buffer one tile ahead, and read by all waves.
 // ALIGN4: block_size % 4 == 0, so four keys from a multiple of four on share a block (one table lookup).
 template <int D, int MODE, int QB, int BN, int WAVES, bool ALIGN4, bool ZS>
-__device__ __forceinline__ void chunk_attn_body(const ChunkArgs &a, int n_slots, int bid) {
+__device__ __forceinline__ void chunk_attn_body(const ChunkArgs &a, int bid) {
     constexpr int DW = D / 4;
     constexpr bool BF8 = MODE == FEATHER_E5M2;
     constexpr int KS = BF8 ? (D + 16) / 2 : D + 8;   // K row pitch in LDS, in fp16 units (bf8: D + 16 bytes)
     constexpr int VS = BN, CH = BN / 8;
     constexpr int kThreads = 64 * WAVES, QT = 16 * QB * WAVES;
     constexpr int UNITS = BN * D / 16;
-    constexpr int NU = UNITS >= kThreads ? UNITS / kThreads : 1;
-    constexpr bool ALL_STAGE = UNITS >= kThreads;
-    static_assert(UNITS % 64 == 0 && (ALL_STAGE ? UNITS % kThreads == 0 : true), "tile / workgroup mismatch");
+    constexpr int NU = UNITS / kThreads;
+    static_assert(UNITS % kThreads == 0 && NU >= 1, "tile / workgroup mismatch");
     constexpr int DB = D / 16, STEPS = D / 32, KB16 = BN / 16, KB32 = BN / 32;
     constexpr int kBufHalfs = BN * KS + D * VS;
 
@@ -270,7 +267,6 @@ __device__ __forceinline__ void chunk_attn_body(const ChunkArgs &a, int n_slots,
     uint32_t vreg[NU][4];
     int kid[NU], vid[NU][ALIGN4 ? 1 : 4];
     auto fetch_ids = [&](int key0) {
-        if (!ALL_STAGE && tid >= UNITS) return;
 #pragma unroll
         for (int i = 0; i < NU; i++) {
             const int u = tid + kThreads * i;
@@ -285,7 +281,6 @@ __device__ __forceinline__ void chunk_attn_body(const ChunkArgs &a, int n_slots,
         return (int64_t)(uint32_t)(min((uint32_t)id, a.max_blk) * (uint32_t)block_rows + (uint32_t)head_rows + slot);
     };
     auto prefetch = [&](int key0) {                    // the ids of this tile are in kid / vid
-        if (!ALL_STAGE && tid >= UNITS) return;
 #pragma unroll
         for (int i = 0; i < NU; i++) {
             const int u = tid + kThreads * i;
@@ -307,7 +302,6 @@ __device__ __forceinline__ void chunk_attn_body(const ChunkArgs &a, int n_slots,
     // NaN.  Such a code is staged as zero: a column that does not see its key has P = 0 there, and 0 * inf is NaN.
     auto stage = [&](int buf, bool diag) -> int {
         int nf = 0;
-        if (!ALL_STAGE && tid >= UNITS) return 0;
         _Float16 *k_lds = lds + buf * kBufHalfs;
         _Float16 *vt_lds = k_lds + BN * KS;
 #pragma unroll
@@ -520,16 +514,15 @@ __device__ __forceinline__ void chunk_attn_body(const ChunkArgs &a, int n_slots,
 typedef int int8p_t __attribute__((ext_vector_type(8)));
 
 template <int D, int MODE, int CB, int WAVES, bool PAGE16, bool ZS>
-__device__ __forceinline__ void chunk_attn32_body(const ChunkArgs &a, int n_slots, int bid) {
+__device__ __forceinline__ void chunk_attn32_body(const ChunkArgs &a, int bid) {
     constexpr bool BF8 = MODE == FEATHER_E5M2;
     constexpr int DW = D / 4, BN = 64, DB = D / 32, STEPS = BF8 ? D / 64 : D / 16;   // 32-dim blocks; matrix steps of a score block
     constexpr int KP = (BF8 ? D : 2 * D) + 16;   // K row pitch in LDS, bytes
     constexpr int VS = BN;                       // fp16 per V^T row
     constexpr int kThreads = 64 * WAVES, QT = 32 * CB * WAVES;
     constexpr int kBufBytes = BN * KP + D * VS * 2;
-    constexpr bool kSplit = D * 16 < 2 * kThreads;   // more threads than a tile has 16-byte units: half of the waves stage K, half V
-    constexpr int UNITS = BN * D / 16, STAGERS = kSplit ? kThreads / 2 : kThreads, NU = UNITS / STAGERS;
-    static_assert(UNITS % STAGERS == 0 && STAGERS % 64 == 0 && NU >= 1, "tile / workgroup mismatch");
+    constexpr int UNITS = BN * D / 16, NU = UNITS / kThreads;
+    static_assert(UNITS % kThreads == 0 && NU >= 1, "tile / workgroup mismatch");
 
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     auto swz = [](int row) { return ((row >> 1) & 7) ^ ((row >> 4) & 1); };   // 16-byte chunk c of V^T row r lives at chunk c ^ swz(r)
@@ -609,24 +602,21 @@ __device__ __forceinline__ void chunk_attn32_body(const ChunkArgs &a, int n_slot
 
     // ---- staging: a thread carries NU units of K (16 bytes of one key) and of V (4 keys x 4 dims); unit u of either is in
     // the keys u / (D / 16) .. of the tile, so the 64 units of a wave lie in 16 neighbouring keys, the same for K and V
-    const bool stages_v = !kSplit || wave < WAVES / 2, stages_k = !kSplit || wave >= WAVES / 2;
-    const int stager = kSplit && wave >= WAVES / 2 ? tid - STAGERS : tid;
-    const int key_wave = (kSplit ? wave % (WAVES / 2) : wave) * (1024 / D);   // the wave's first key of its first units
-    constexpr int kKeysPerTurn = STAGERS * 16 / D;
+    const int key_wave = wave * (1024 / D);      // the wave's first key of its first units
+    constexpr int kKeysPerTurn = kThreads * 16 / D;
     const __attribute__((address_space(4))) int32_t *bt_const = (const __attribute__((address_space(4))) int32_t *)bt;   // read only while the kernel runs: scalar loads
     int id_k[NU], id_v[PAGE16 ? 1 : NU][PAGE16 ? 1 : 4];   // PAGE16: id_k only, wave-uniform
     auto first16 = [&](int key0, int i) { return min((key0 + key_wave + kKeysPerTurn * i) & ~15, (key_end - 1) & ~15); };
     auto fetch_ids = [&](int key0) {
 #pragma unroll
         for (int i = 0; i < NU; i++) {
-            const int u = stager + STAGERS * i;
+            const int u = tid + kThreads * i;
             if constexpr (PAGE16) {
                 id_k[i] = bt_const[chunk_block_of(a, first16(key0, i))];
             } else {
-                if (stages_k) id_k[i] = bt[chunk_block_of(a, min(key0 + u / (D / 16), key_end - 1))];
-                if (stages_v)
+                id_k[i] = bt[chunk_block_of(a, min(key0 + u / (D / 16), key_end - 1))];
 #pragma unroll
-                    for (int r = 0; r < 4; r++) id_v[i][r] = bt[chunk_block_of(a, min(key0 + 4 * (u / DW) + r, key_end - 1))];
+                for (int r = 0; r < 4; r++) id_v[i][r] = bt[chunk_block_of(a, min(key0 + 4 * (u / DW) + r, key_end - 1))];
             }
         }
     };
@@ -635,21 +625,18 @@ __device__ __forceinline__ void chunk_attn32_body(const ChunkArgs &a, int n_slot
     auto prefetch = [&](int key0) {              // keys past the end: another key's row (masked; its V is zeroed by `stage`)
 #pragma unroll
         for (int i = 0; i < NU; i++) {
-            const int u = stager + STAGERS * i;
+            const int u = tid + kThreads * i;
             if constexpr (PAGE16) {
                 const int pos = first16(key0, i);
-                if (stages_k) kreg[i] = *reinterpret_cast<const u32x4 *>(row_at(a.k_cache, id_k[i], pos) + (uint32_t)((u / (D / 16) % 16) * D + 16 * (u % (D / 16))));
-                if (stages_v) {
-                    const char *vr = row_at(a.v_cache, id_k[i], pos) + (uint32_t)((u / DW % 4) * 4 * D + 4 * (u % DW));
+                kreg[i] = *reinterpret_cast<const u32x4 *>(row_at(a.k_cache, id_k[i], pos) + (uint32_t)((u / (D / 16) % 16) * D + 16 * (u % (D / 16))));
+                const char *vr = row_at(a.v_cache, id_k[i], pos) + (uint32_t)((u / DW % 4) * 4 * D + 4 * (u % DW));
 #pragma unroll
-                    for (int r = 0; r < 4; r++) vreg[i][r] = *reinterpret_cast<const uint32_t *>(vr + r * D);
-                }
+                for (int r = 0; r < 4; r++) vreg[i][r] = *reinterpret_cast<const uint32_t *>(vr + r * D);
             } else {
-                if (stages_k) kreg[i] = *reinterpret_cast<const u32x4 *>(row_at(a.k_cache, id_k[i], min(key0 + u / (D / 16), key_end - 1)) + 16 * (u % (D / 16)));
-                if (stages_v)
+                kreg[i] = *reinterpret_cast<const u32x4 *>(row_at(a.k_cache, id_k[i], min(key0 + u / (D / 16), key_end - 1)) + 16 * (u % (D / 16)));
 #pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        vreg[i][r] = *reinterpret_cast<const uint32_t *>(row_at(a.v_cache, id_v[i][r], min(key0 + 4 * (u / DW) + r, key_end - 1)) + 4 * (u % DW));
+                for (int r = 0; r < 4; r++)
+                    vreg[i][r] = *reinterpret_cast<const uint32_t *>(row_at(a.v_cache, id_v[i][r], min(key0 + 4 * (u / DW) + r, key_end - 1)) + 4 * (u % DW));
             }
         }
     };
@@ -662,54 +649,50 @@ __device__ __forceinline__ void chunk_attn32_body(const ChunkArgs &a, int n_slot
         _Float16 *vt_lds = reinterpret_cast<_Float16 *>(k_lds + BN * KP);
 #pragma unroll
         for (int i = 0; i < NU; i++) {
-            const int u = stager + STAGERS * i;
-            if (stages_k) {
-                const int key = u / (D / 16), c16 = u % (D / 16);
-                if constexpr (BF8) {
-                    *reinterpret_cast<u32x4 *>(k_lds + key * KP + 16 * c16) = kreg[i];
-                } else {
-                    half8_t *kd = reinterpret_cast<half8_t *>(k_lds + key * KP + 32 * c16);
-                    kd[0] = chunk_dec8<MODE>(kreg[i].x, kreg[i].y);
-                    kd[1] = chunk_dec8<MODE>(kreg[i].z, kreg[i].w);
-                }
+            const int u = tid + kThreads * i;
+            const int key = u / (D / 16), c16 = u % (D / 16);
+            if constexpr (BF8) {
+                *reinterpret_cast<u32x4 *>(k_lds + key * KP + 16 * c16) = kreg[i];
+            } else {
+                half8_t *kd = reinterpret_cast<half8_t *>(k_lds + key * KP + 32 * c16);
+                kd[0] = chunk_dec8<MODE>(kreg[i].x, kreg[i].y);
+                kd[1] = chunk_dec8<MODE>(kreg[i].z, kreg[i].w);
             }
-            if (stages_v) {
-                const int ddw = u % DW, kg = u / DW;
-                const int q4 = kg & 3, pos = 16 * (kg >> 2) + 8 * (q4 & 1) + 4 * (q4 >> 1);
-                uint32_t (&w)[4] = vreg[i];
-                if (key0 + BN > key_end)
+            const int ddw = u % DW, kg = u / DW;
+            const int q4 = kg & 3, pos = 16 * (kg >> 2) + 8 * (q4 & 1) + 4 * (q4 >> 1);
+            uint32_t (&w)[4] = vreg[i];
+            if (key0 + BN > key_end)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) w[r] = key0 + 4 * kg + r < key_end ? w[r] : 0u;
-                uint32_t lo2[4], hi2[4];         // halfs (key 0, key 1) and (key 2, key 3) of dim 4 ddw + c
-                if constexpr (BF8) {
-                    if (on_diag(key0)) {
+                for (int r = 0; r < 4; r++) w[r] = key0 + 4 * kg + r < key_end ? w[r] : 0u;
+            uint32_t lo2[4], hi2[4];         // halfs (key 0, key 1) and (key 2, key 3) of dim 4 ddw + c
+            if constexpr (BF8) {
+                if (on_diag(key0)) {
 #pragma unroll
-                        for (int r = 0; r < 4; r++) {
-                            const uint32_t m = chunk_nonfinite(w[r]);
-                            w[r] &= ~m;
-                            nf |= m != 0;
-                        }
+                    for (int r = 0; r < 4; r++) {
+                        const uint32_t m = chunk_nonfinite(w[r]);
+                        w[r] &= ~m;
+                        nf |= m != 0;
                     }
-#pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        const uint32_t sel = 0x000c000cu | ((uint32_t)c << 8) | ((uint32_t)(4 + c) << 24);
-                        lo2[c] = perm(w[1], w[0], sel);
-                        hi2[c] = perm(w[3], w[2], sel);
-                    }
-                } else {
-                    uint32_t p01[4], p23[4];
-#pragma unroll
-                    for (int r = 0; r < 4; r++) dec_word<MODE>(w[r], p01[r], p23[r]);
-                    lo2[0] = perm(p01[1], p01[0], 0x05040100u); hi2[0] = perm(p01[3], p01[2], 0x05040100u);
-                    lo2[1] = perm(p01[1], p01[0], 0x07060302u); hi2[1] = perm(p01[3], p01[2], 0x07060302u);
-                    lo2[2] = perm(p23[1], p23[0], 0x05040100u); hi2[2] = perm(p23[3], p23[2], 0x05040100u);
-                    lo2[3] = perm(p23[1], p23[0], 0x07060302u); hi2[3] = perm(p23[3], p23[2], 0x07060302u);
                 }
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    const int row = 4 * ddw + c;
-                    *reinterpret_cast<u32x2 *>(vt_lds + row * VS + (((pos >> 3) ^ swz(row)) << 3) + (pos & 4)) = u32x2{lo2[c], hi2[c]};
+                    const uint32_t sel = 0x000c000cu | ((uint32_t)c << 8) | ((uint32_t)(4 + c) << 24);
+                    lo2[c] = perm(w[1], w[0], sel);
+                    hi2[c] = perm(w[3], w[2], sel);
                 }
+            } else {
+                uint32_t p01[4], p23[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) dec_word<MODE>(w[r], p01[r], p23[r]);
+                lo2[0] = perm(p01[1], p01[0], 0x05040100u); hi2[0] = perm(p01[3], p01[2], 0x05040100u);
+                lo2[1] = perm(p01[1], p01[0], 0x07060302u); hi2[1] = perm(p01[3], p01[2], 0x07060302u);
+                lo2[2] = perm(p23[1], p23[0], 0x05040100u); hi2[2] = perm(p23[3], p23[2], 0x05040100u);
+                lo2[3] = perm(p23[1], p23[0], 0x07060302u); hi2[3] = perm(p23[3], p23[2], 0x07060302u);
+            }
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const int row = 4 * ddw + c;
+                *reinterpret_cast<u32x2 *>(vt_lds + row * VS + (((pos >> 3) ^ swz(row)) << 3) + (pos & 4)) = u32x2{lo2[c], hi2[c]};
             }
         }
         return nf;
@@ -1368,16 +1351,16 @@ constexpr size_t narrow_lds(int d, int nb, int ring) {   // the rings, or the ex
 }
 
 template <int D, int MODE, bool PAGE16, bool ZS>
-__device__ __forceinline__ void chunk_wide_body(const ChunkArgs &a, int n_slots, int bid) {
+__device__ __forceinline__ void chunk_wide_body(const ChunkArgs &a, int bid) {
     constexpr WideShape w = wide_shape(D);
-    if constexpr (D <= kMost32) chunk_attn32_body<D, MODE, w.columns / (32 * w.waves), w.waves, PAGE16, ZS>(a, n_slots, bid);
-    else chunk_attn_body<D, MODE, w.columns / (16 * w.waves), w.keys, w.waves, PAGE16, ZS>(a, n_slots, bid);
+    if constexpr (D <= kMost32) chunk_attn32_body<D, MODE, w.columns / (32 * w.waves), w.waves, PAGE16, ZS>(a, bid);
+    else chunk_attn_body<D, MODE, w.columns / (16 * w.waves), w.keys, w.waves, PAGE16, ZS>(a, bid);
 }
 
 template <int D, int MODE, bool PAGE16, bool ZS>
 __global__ __launch_bounds__(64 * wide_shape(D).waves, wide_shape(D).occ) void chunk_wide_kernel(ChunkArgs a, int n_slots) {
     const int work = n_slots * a.n_kv_heads * (ZS ? a.z_wide : 1), bid = blockIdx.x;
-    if (bid < work) chunk_wide_body<D, MODE, PAGE16, ZS>(a, n_slots, bid);
+    if (bid < work) chunk_wide_body<D, MODE, PAGE16, ZS>(a, bid);
     else chunk_fill_outside<D>(a, bid - work, gridDim.x - work, 64 * wide_shape(D).waves);
 }
 
@@ -1395,7 +1378,7 @@ __global__ __launch_bounds__(256, wide_shape(D).occ) void chunk_mixed_kernel(Chu
     int bid = blockIdx.x;
     const int wide = n_slots * a.n_kv_heads * (ZS ? a.z_wide : 1), pairs = a.n_seq * a.n_kv_heads, narrow = pairs * a.z_narrow;
     if (bid < wide) {
-        chunk_wide_body<D, MODE, PAGE16, ZS>(a, n_slots, bid);
+        chunk_wide_body<D, MODE, PAGE16, ZS>(a, bid);
         return;
     }
     bid -= wide;
@@ -1559,7 +1542,7 @@ static ChunkPlan chunk_plan(int64_t n_seq, int64_t total_rows, int64_t n_q_heads
         // with n_seq - 1 sequences of the longest length, can the last one be short?  (If the hint is wrong the LDS kernel
         // takes the short ones too.)
         const int64_t least = total_rows - (n_seq - 1) * rows_most;
-        p.narrow = n_seq > 1 && (least < 0 ? 0 : least) * group <= 16 * p.nb;
+        p.narrow = n_seq > 1 && (least < 1 ? 1 : least) * group <= 16 * p.nb;   // (one row has `group` columns)
         p.col_split = p.narrow ? 16 * p.nb : 0;
     }
     p.narrow_rows = p.wide && p.narrow ? (int)(p.col_split / group) : 0;

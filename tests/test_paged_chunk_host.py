@@ -39,6 +39,8 @@ def test_chunk_attention_argument_checks():
             for d in (64, 128, 256, 512):
                 for hint in (0, 1, 64, rows):
                     assert size(n_seq, rows, 32, 4, d, 1 << 20, hint) < 1 << 30
+    for d in (64, 128, 256, 512):                                           # a row of more columns than a narrow tile has: no
+        assert size(16, 4111, 64, 1, d, 1 << 20, 4096) < 1 << 30            # sequence is short, none gets room for one
 
 
 def test_rope_chunk_argument_checks():
