@@ -139,6 +139,8 @@ def paged_chunk_attention_fp8_acc_fp32_gpu(q: torch.Tensor, k_cache: torch.Tenso
     elif (not isinstance(out, torch.Tensor) or out.dtype != out_dtype or tuple(out.shape) != shape
           or out.device != dev or not out.is_contiguous()):
         raise ValueError(f"out must be a contiguous {out_dtype} tensor of shape {shape} on {dev}")
+    elif any(t.data_ptr() < out.data_ptr() + out.nbytes and out.data_ptr() < t.data_ptr() + t.nbytes for t in (q, k_cache, v_cache)):
+        raise ValueError("out overlaps q or a cache, which are read while it is written")
     block_tables, cu_seqlens, ctx_lens = block_tables.contiguous(), cu_seqlens.contiguous(), ctx_lens.contiguous()
     max_blocks = block_tables.shape[1]
     lib = N.lib()

@@ -47,12 +47,13 @@ def _pool(caches, ref_counts: torch.Tensor):
         raise ValueError(f"caches must be uint32/int32/float32 containers, got {dtypes}")
     if not whole or first.dim() != 4:
         raise ValueError("caches are updated in place: expected contiguous [n_blocks, n_kv_heads, block_size, d/4]")
-    if len(set(ptrs)) != len(ptrs):
-        raise ValueError("caches holds the same tensor twice")
     n_blocks, n_kv, block_size, dw = first.shape
     block_bytes = 4 * n_kv * block_size * dw
     if block_bytes == 0 or block_bytes % 16 != 0:
         raise ValueError(f"a block of {block_bytes} bytes is not a multiple of 16")
+    ordered = sorted(ptrs)
+    if min(map(operator.sub, ordered[1:], ordered), default=n_blocks * block_bytes) < n_blocks * block_bytes:
+        raise ValueError("caches overlap (or the same tensor is there twice)")
     if ref_counts.shape != (n_blocks,) or n_blocks < 1:
         raise ValueError(f"ref_counts must be [n_blocks={n_blocks}] with at least one block")
     if ref_counts.device != first.device:

@@ -261,3 +261,15 @@ def test_refusals(dev):
     t, c, r, s = paged_cache_fork([k, v], i32(2, 0), i32(2), i32(6), i32(2))           # a table without entries
     assert s.cpu().tolist() == [0, 0] and c.cpu().tolist() == [0, 0]
     assert paged_cache_compact([k], i32(0, 3), i32(6))[3].item() == 0
+
+
+def test_overlapping_caches_are_refused():
+    from feather_amd.routines.paged_cache import paged_cache_compact
+    pool = torch.zeros((9, 2, 16, 16), dtype=torch.int32, device="cuda")
+    tables, ref = torch.zeros((1, 2), dtype=torch.int32, device="cuda"), torch.zeros(8, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="overlap"):
+        paged_cache_compact([pool[:8], pool[1:]], tables, ref)
+    with pytest.raises(ValueError, match="overlap"):
+        paged_cache_compact([pool[:8], pool[:8]], tables, ref)
+    both = torch.zeros((2, 8, 2, 16, 16), dtype=torch.int32, device="cuda")
+    paged_cache_compact([both[1], both[0]], tables, ref)       # side by side is fine

@@ -317,3 +317,15 @@ def test_cross_attention_over_a_longer_and_a_shorter_state(dev, orc):
     P = _problem(orc, 10, [77, 300], [500, 21], 4, 4, 128, 16, "E4M3")
     y, tol = _reference(P, orc, False, scale=0.2)
     _check(_call(P, dev, False, scale=0.2), y, tol)
+
+
+def test_out_that_overlaps_an_input_is_refused():
+    from feather_amd.routines.paged_attention import paged_chunk_attention_fp8_acc_fp32_gpu
+    z = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")
+    q, kc, cu, ctx, tables = z(3, 4, 16), z(4, 2, 16, 16), z(2), z(1), z(1, 2)
+    with pytest.raises(ValueError, match="overlaps"):
+        paged_chunk_attention_fp8_acc_fp32_gpu(q, kc, kc.clone(), tables, cu, ctx, out_dtype=torch.uint32,
+                                               out=q.view(3, 64).view(torch.uint32))
+    with pytest.raises(ValueError, match="overlaps"):
+        paged_chunk_attention_fp8_acc_fp32_gpu(q, kc, kc.clone(), tables, cu, ctx, out_dtype=torch.uint32,
+                                               out=kc.view(-1)[64:256].view(3, 64).view(torch.uint32))
