@@ -16,6 +16,10 @@ import torch
 
 from .. import _native as N
 from ..packers.fp8 import pack_fp8_tensor
+from .gemv import gemv_fp8_batched_acc_fp32_gpu
+from .paged_attention import paged_chunk_attention_fp8_acc_fp32_gpu
+from .paged_cache import paged_cache_compact, paged_cache_fork
+from .producers import add_rmsnorm_pack, gemv_fp8_batched_swiglu, rope_append_chunk, rotary_frequencies
 
 __all__ = ["DecoderConfig", "PackedDecoder", "TINYLLAMA_1_1B"]
 
@@ -91,6 +95,7 @@ class PackedDecoder:
                             ctypes.cast(self._c_layers, ctypes.POINTER(N.DecoderLayer)), self.embed.data_ptr(),
                             self.norm_final.data_ptr(), self.lm_head.data_ptr())
         self._scratch = {}
+        self._freq = rotary_frequencies(cfg.head_dim, theta=cfg.rope_theta, device=dev)
 
     def weight_bytes(self) -> int:
         """Packed weight bytes one step streams (each linear layer once, embedding rows aside)."""
@@ -155,6 +160,81 @@ class PackedDecoder:
         N.call(self.device, "feather_decode_step", ctypes.addressof(self._c), N.ptr(token_ids), N.ptr(block_tables),
                N.ptr(ctx_lens), batch, max_ctx, sptr, N.ptr(out), N.ptr(status) if status is not None else None)
         return out
+
+    def extend(self, token_ids: torch.Tensor, cu_seqlens: torch.Tensor, block_tables: torch.Tensor, ctx_lens: torch.Tensor,
+               *, rows: torch.Tensor | None = None, max_q_len: int | None = None):
+        """Run a ragged batch of new tokens through the model: a chunk of a prompt, drafted tokens to verify, or single
+        tokens beside them.
+
+        token_ids     ``[total_rows]`` int32; sequence ``s`` brings ``token_ids[cu[s] : cu[s+1]]``
+        block_tables  ``[n_seq, max_blocks]`` int32; must have blocks for the new tokens, and no two sequences may share
+                      a block that one of them writes (:meth:`fork` with ``room`` sees to both)
+        ctx_lens      ``[n_seq]`` int32 tokens already cached; the new ones get the positions behind them
+        rows          int32 rows whose logits are wanted (default: the last row of each sequence)
+        max_q_len     a bound of a sequence's rows, if known; it only helps to choose the kernels
+        Returns ``(logits, ctx_after [n_seq], status [n_seq])``: float32 logits ``[len(rows), vocab]``, and lengths and
+        status as :func:`rope_append_chunk` gives them.  The logits of a sequence whose status is not 0, and of a
+        sequence without rows, are meaningless.  The linear layers run as batched GEMVs of 64 rows, which suits
+        drafts and short chunks; a long prompt reads the weights once per 64 rows."""
+        cfg = self.cfg
+        if cfg.hidden % 256 != 0 or cfg.head_dim not in (64, 128, 256, 512) or cfg.n_layers < 1:
+            raise ValueError("extend needs hidden to be a multiple of 256, head_dim 64, 128, 256 or 512, and at least one layer")
+        for t, name in ((token_ids, "token_ids"), (cu_seqlens, "cu_seqlens"), (block_tables, "block_tables"),
+                        (ctx_lens, "ctx_lens"), (rows, "rows")):
+            if t is None:
+                continue
+            if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous int32 tensor on the device")
+            if t.device != self.device:
+                raise ValueError(f"{name} is on {t.device}, the decoder on {self.device}")
+        if token_ids.dim() != 1 or token_ids.numel() < 1 or ctx_lens.dim() != 1 or ctx_lens.numel() < 1:
+            raise ValueError("token_ids must be [total_rows >= 1] and ctx_lens [n_seq >= 1]")
+        total, n_seq = token_ids.numel(), ctx_lens.numel()
+        if block_tables.shape != (n_seq, self.max_blocks) or cu_seqlens.shape != (n_seq + 1,):
+            raise ValueError("block_tables must be [n_seq, max_blocks] and cu_seqlens [n_seq + 1]")
+        if rows is not None and rows.dim() != 1:
+            raise ValueError("rows must be a list of row numbers")
+
+        def slices(f, x):
+            parts = [f(x[i:i + 64], min(64, x.shape[0] - i)) for i in range(0, x.shape[0], 64)]
+            if len(parts) == 1:
+                return parts[0]
+            return torch.cat([p.view(torch.int32) if p.dtype == torch.uint32 else p for p in parts])
+
+        def linear(w, x, n_out):
+            return slices(lambda p, n: gemv_fp8_batched_acc_fp32_gpu(w, p, (n_out, 4 * x.shape[1]), n, self.mode), x)
+
+        h = self.embed[token_ids.clamp(0, cfg.vocab - 1)].float()
+        delta = None
+        for lay in self.layers:
+            x = add_rmsnorm_pack(h, lay["norm_attn"], delta, eps=cfg.rms_eps, mode=self.mode)
+            q, ctx_after, status = rope_append_chunk(linear(lay["w_qkv"], x, cfg.qkv_rows), cu_seqlens, ctx_lens, block_tables,
+                                                     lay["k_cache"], lay["v_cache"], n_q_heads=cfg.n_q_heads, freq=self._freq,
+                                                     mode=self.mode)
+            att = paged_chunk_attention_fp8_acc_fp32_gpu(q, lay["k_cache"], lay["v_cache"], block_tables, cu_seqlens, ctx_after,
+                                                         mode=self.mode, max_q_len=max_q_len, out_dtype=torch.uint32)
+            x = add_rmsnorm_pack(h, lay["norm_mlp"], linear(lay["w_o"], att, cfg.hidden)[None], eps=cfg.rms_eps, mode=self.mode)
+            act = slices(lambda p, n: gemv_fp8_batched_swiglu(lay["w_gate_up"], p, cfg.inter, cfg.hidden, n, mode=self.mode), x)
+            delta = linear(lay["w_down"], act, cfg.hidden)[None]
+        x = add_rmsnorm_pack(h, self.norm_final, delta, eps=cfg.rms_eps, mode=self.mode)
+        if rows is None:
+            rows = cu_seqlens[1:] - 1
+        x = x.view(torch.int32)[rows.clamp(0, total - 1)]
+        if x.shape[0] == 0:
+            return h.new_empty((0, cfg.vocab)), ctx_after, status
+        return linear(self.lm_head, x, cfg.vocab), ctx_after, status
+
+    def _caches(self):
+        return [lay[name] for lay in self.layers for name in ("k_cache", "v_cache")]
+
+    def fork(self, block_tables: torch.Tensor, ctx_lens: torch.Tensor, ref_counts: torch.Tensor, parents: torch.Tensor, *,
+             room: torch.Tensor | None = None):
+        """:func:`paged_cache_fork` over the caches of all layers: slot ``i`` goes on as a copy of slot ``parents[i]``."""
+        return paged_cache_fork(self._caches(), block_tables, ctx_lens, ref_counts, parents, room=room)
+
+    def compact(self, block_tables: torch.Tensor, ref_counts: torch.Tensor):
+        """:func:`paged_cache_compact` over the caches of all layers."""
+        return paged_cache_compact(self._caches(), block_tables, ref_counts)
 
 
 def random_weights(cfg: DecoderConfig, seed: int = 5, device="cpu") -> dict:
