@@ -251,17 +251,16 @@ __device__ __forceinline__ void chunk_attn_body(const ChunkArgs &a, int bid) {
             else qf[b][s] = chunk_dec8<MODE>(w.x, w.y);
         }
 
-    float4_t o[QB][DB + 1];          // [DB]: row sums of P, from a constant block of ones
-    float m_run[QB];
+    float4_t o[QB][DB];
+    float m_run[QB], l_run[QB];      // reference point, the lane's share of the sum
 #pragma unroll
     for (int b = 0; b < QB; b++) {
         m_run[b] = -INFINITY;
+        l_run[b] = 0.f;
 #pragma unroll
-        for (int d = 0; d <= DB; d++) o[b][d] = float4_t{0.f, 0.f, 0.f, 0.f};
+        for (int d = 0; d < DB; d++) o[b][d] = float4_t{0.f, 0.f, 0.f, 0.f};
     }
     const float lazy_raw = 8.f / a.scale_log2e;
-    const _Float16 one_or_zero = (j & 3) == 0 ? (_Float16)1 : (_Float16)0;
-    const half8_t ones = {one_or_zero, one_or_zero, one_or_zero, one_or_zero, one_or_zero, one_or_zero, one_or_zero, one_or_zero};
 
     u32x4 kreg[NU];
     uint32_t vreg[NU][4];
@@ -426,34 +425,35 @@ __device__ __forceinline__ void chunk_attn_body(const ChunkArgs &a, int bid) {
                 const bool raise = __builtin_amdgcn_ballot_w64(mx > m_old + lazy_raw) != 0;
                 const float m_new = raise ? max_raw(m_old, mx) : m_old;
                 const float mc = m_new == -INFINITY ? 0.f : m_new * a.scale_log2e;
-#pragma unroll
-                for (int g = 0; g < KB32; g++) {
-                    half8_t p8;
-#pragma unroll
-                    for (int h = 0; h < 2; h++)
-#pragma unroll
-                        for (int r = 0; r < 4; r++)
-                            p8[4 * h + r] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[b][2 * g + h][r], a.scale_log2e, -mc));
-                    pf[b][g] = p8;
-                }
                 if (raise) {
                     const float alpha = m_old == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_old - m_new) * a.scale_log2e);
                     m_run[b] = m_new;
+                    l_run[b] *= alpha;
 #pragma unroll
-                    for (int d = 0; d <= DB; d++) o[b][d] *= alpha;
+                    for (int d = 0; d < DB; d++) o[b][d] *= alpha;
+                }
+#pragma unroll
+                for (int g = 0; g < KB32; g++) {
+                    uint32_t pw[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float4_t &x = s[b][2 * g + (i >> 1)];
+                        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * (i & 1)], a.scale_log2e, -mc));
+                        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * (i & 1) + 1], a.scale_log2e, -mc));
+                        pw[i] = as_u32(__builtin_convertvector(float2p_t{e0, e1}, half2_t));
+                        l_run[b] = dot2(pw[i], 0x3c003c00u, l_run[b]);   // the sum takes the rounded values that multiply V
+                    }
+                    pf[b][g] = __builtin_bit_cast(half8_t, u32x4{pw[0], pw[1], pw[2], pw[3]});
                 }
             }
 #pragma unroll
-            for (int g = 0; g < KB32; g++) {
+            for (int g = 0; g < KB32; g++)
 #pragma unroll
                 for (int d = 0; d < DB; d++) {
                     const half8_t vf = *reinterpret_cast<const half8_t *>(vt_lds + (16 * d + j) * VS + (((4 * g + kb) ^ swz(16 * d + j)) << 3));
 #pragma unroll
                     for (int b = 0; b < QB; b++) o[b][d] = chunk_mfma16(vf, pf[b][g], o[b][d]);
                 }
-#pragma unroll
-                for (int b = 0; b < QB; b++) o[b][DB] = chunk_mfma16(ones, pf[b][g], o[b][DB]);
-            }
             if (BF8 && nf) {   // rare: what the staged zeros stand for, added for the columns that see the key
                 for (int key = key0; key < min(key0 + BN, key_end); key++) {
                     const uint32_t *vr = a.v_cache + row_of(bt[chunk_block_of(a, key)], key) * DW + kb;
@@ -487,8 +487,10 @@ __device__ __forceinline__ void chunk_attn_body(const ChunkArgs &a, int bid) {
     if (!wave_has) return;
 #pragma unroll
     for (int b = 0; b < QB; b++) {
+        float l = l_run[b];
+        l += __shfl_xor(l, 16, kWave);
+        l += __shfl_xor(l, 32, kWave);
         if (qc0 + 16 * b + j >= t.cols) continue;
-        const float l = o[b][DB][0];
         if constexpr (ZS) {
             const int64_t items = (int64_t)a.total_rows * a.n_q_heads, at = zr * items + item[b];
 #pragma unroll
@@ -1335,7 +1337,7 @@ __device__ __forceinline__ void chunk_narrow_body(const ChunkArgs &a, int pair, 
 struct WideShape { int columns, waves, keys, occ; };
 constexpr int kMost32 = 128;             // largest head dim on the 32x32 instructions
 static constexpr WideShape wide_shape(int64_t d) {
-    return d == 64 ? WideShape{256, 4, 64, 2} : (d == 128 ? WideShape{128, 4, 64, 2} : (d == 256 ? WideShape{128, 8, 64, 1} : WideShape{64, 4, 32, 1}));
+    return d == 64 ? WideShape{256, 4, 64, 2} : (d == 128 ? WideShape{128, 4, 64, 2} : (d == 256 ? WideShape{128, 8, 64, 1} : WideShape{128, 8, 32, 1}));
 }
 // Steps in the ring of a wave of the narrow kernel (0: the rows go through registers).
 static constexpr int ring_steps(int d, int nb) { return d == 64 ? 4 : (d == 128 ? (nb == 4 ? 4 : 2) : (d == 256 ? 2 : 0)); }
