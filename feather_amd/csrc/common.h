@@ -299,16 +299,6 @@ __device__ __forceinline__ float max3_raw(float a, float b, float c) {
     return r;
 }
 
-// sin and cos of q * pi/2 + r for r in [-pi/4, pi/4]: single-precision minimax polynomials and the quadrant's signs
-__device__ __forceinline__ void sincos_quadrant(float r, int q, float &s, float &c) {
-    const float r2 = r * r;
-    const float sp = fmaf(r * r2, fmaf(r2, fmaf(r2, -1.9515295891e-4f, 8.3321608736e-3f), -1.6666654611e-1f), r);
-    const float cp = fmaf(r2, fmaf(r2, fmaf(r2, fmaf(r2, 2.443315711809948e-5f, -1.388731625493765e-3f), 4.166664568298827e-2f), -0.5f), 1.0f);
-    const float ss = (q & 1) ? cp : sp, cc = (q & 1) ? sp : cp;
-    s = (q & 2) ? -ss : ss;
-    c = ((q + 1) & 2) ? -cc : cc;
-}
-
 __device__ __forceinline__ int lane_id() { return (int)(threadIdx.x & (kWave - 1)); }
 
 // Index of the wave inside its workgroup, marked as wave-uniform: everything derived from it (row

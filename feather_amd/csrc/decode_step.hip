@@ -201,7 +201,13 @@ __device__ __forceinline__ void sincos_small(float x, float &s, float &c) {
     float r = fmaf(k, -1.57079625e+00f, x);
     r = fmaf(k, -7.54978942e-08f, r);
     r = fmaf(k, -5.39030295e-15f, r);
-    sincos_quadrant(r, (int)k, s, c);
+    const float r2 = r * r;
+    const float sp = fmaf(r * r2, fmaf(r2, fmaf(r2, -1.9515295891e-4f, 8.3321608736e-3f), -1.6666654611e-1f), r);
+    const float cp = fmaf(r2, fmaf(r2, fmaf(r2, fmaf(r2, 2.443315711809948e-5f, -1.388731625493765e-3f), 4.166664568298827e-2f), -0.5f), 1.0f);
+    const int q = (int)k;
+    const float ss = (q & 1) ? cp : sp, cc = (q & 1) ? sp : cp;
+    s = (q & 2) ? -ss : ss;
+    c = ((q + 1) & 2) ? -cc : cc;
 }
 
 // (parameter order: everything needed before the first loads sits in the 16 preloaded dwords)

@@ -15,6 +15,17 @@ namespace feather {
 constexpr int kRcThreads = 256;
 constexpr int kRcMaxPairs = 256;      // rot_dim <= 512
 
+// sin and cos of q * pi/2 + r for r in [-pi/4, pi/4]: single-precision minimax polynomials (the decode step's) and the
+// quadrant's signs
+__device__ __forceinline__ void sincos_quadrant(float r, int q, float &s, float &c) {
+    const float r2 = r * r;
+    const float sp = fmaf(r * r2, fmaf(r2, fmaf(r2, -1.9515295891e-4f, 8.3321608736e-3f), -1.6666654611e-1f), r);
+    const float cp = fmaf(r2, fmaf(r2, fmaf(r2, fmaf(r2, 2.443315711809948e-5f, -1.388731625493765e-3f), 4.166664568298827e-2f), -0.5f), 1.0f);
+    const float ss = (q & 1) ? cp : sp, cc = (q & 1) ? sp : cp;
+    s = (q & 2) ? -ss : ss;
+    c = ((q + 1) & 2) ? -cc : cc;
+}
+
 struct RopeChunkArgs {
     const void *qkv;
     const int32_t *cu_seqlens, *start_pos, *block_tables;
