@@ -16,6 +16,20 @@
 // (nearest even) before it multiplies V, as in the other attention kernels: the second product then runs at the fp16
 // rate, and the error (2^-11 / sqrt(3) of each P, random in sign) is of the size of the fp16 result's own rounding.
 // The denominator sums the rounded P.
+//
+// Kernels.  Many columns: K and V tiles through LDS, shared by a workgroup's waves -- chunk_attn32_body (d = 64, 128) on
+// the 32x32 matrix instructions, chunk_attn_body (d = 256, 512) on the 16x16 ones.  Few columns: chunk_narrow_body, where
+// the bytes of the cache bound the call.  A batch that has both runs both, in one grid where the workgroups are alike.
+// Key ranges share a column out over more workgroups, chunk_merge_kernel adds them up.
+//
+// Measured (a chunk of 2048 rows whose last key is 8192, causal; products and sums of the visible keys, merge included):
+//     d = 64, 32 heads on 4    E5M2 147 + 11 us, 760 TFLOP/s    E4M3 175 + 11 us, 650 TFLOP/s
+//     d = 128, 32 on 8         E5M2 243 us, 990 TFLOP/s         E4M3 317 us, 760 TFLOP/s
+//     d = 256, 8 on 8          E5M2 210 + 14 us, 540 TFLOP/s    E4M3 217 + 14 us, 520 TFLOP/s
+//     d = 512, 8 on 8          E5M2 425 + 26 us, 530 TFLOP/s    E4M3 543 + 26 us, 420 TFLOP/s
+// (a plain fp16 product of 8192^3 on the same card: 1168).  Bound: vector issue beside the matrix cores up to d = 128 (the
+// exponentials, the decode); LDS reads from d = 256 on (16 columns per wave read every K and V tile once per wave: twice
+// the time of the products), which more columns per wave would halve if the accumulators left registers for them.
 #include <type_traits>
 
 #include "common.h"
@@ -152,7 +166,10 @@ __device__ __forceinline__ void chunk_fill_outside(const ChunkArgs &a, int part,
 }
 
 constexpr int kChunkFillGroups = 8;    // workgroups of a grid that only look after rows outside every sequence
-constexpr int kChunkMinKeys = 256;     // a key range is not cut below this (LDS kernel / narrow kernel)
+// A key range is not cut below this.  LDS kernel: 3 x 97 to 203 rows over 750 to 1501 keys, d = 256: 128 keys 34.5 + 7.6 us
+// (kernel, merge), 256 keys 28.6 + 6.2, 512 keys 37.8 + 4.8.  Narrow kernel: two requests of 211 to 300 keys are done in
+// one range and one launch, 9.9 us; with ranges of 256 keys 8.5 + 4.2.
+constexpr int kChunkMinKeys = 256;
 constexpr int kNarrowMinKeys = 512;
 constexpr int kNarrowStep = 128;       // keys that the four waves of a narrow workgroup take per turn
 
@@ -181,8 +198,8 @@ constexpr int kAnyColumns = 1 << 30;   // more columns than a call can have
 // One workgroup (WAVES waves) owns 16 * QB * WAVES columns, each wave 16 * QB of them for the whole key loop.  Tiles
 // of BN keys are fetched packed through the block table into registers two tiles ahead (their block ids three tiles
 // ahead: a table entry is never waited for), decoded into the other LDS buffer one tile ahead, and read by all waves.
-// ALIGN4: block_size % 4 == 0, so four keys from a multiple of four on share a block (one table lookup).
-template <int D, int MODE, int QB, int BN, int WAVES, bool ALIGN4, bool ZS>
+// PAGE4: block_size % 4 == 0, so four keys from a multiple of four on share a block (one table lookup).
+template <int D, int MODE, int QB, int BN, int WAVES, bool PAGE4, bool ZS>
 __device__ __forceinline__ void chunk_attn_body(const ChunkArgs &a, int bid) {
     constexpr int DW = D / 4;
     constexpr bool BF8 = MODE == FEATHER_E5M2;
@@ -264,14 +281,14 @@ __device__ __forceinline__ void chunk_attn_body(const ChunkArgs &a, int bid) {
 
     u32x4 kreg[NU];
     uint32_t vreg[NU][4];
-    int kid[NU], vid[NU][ALIGN4 ? 1 : 4];
+    int kid[NU], vid[NU][PAGE4 ? 1 : 4];
     auto fetch_ids = [&](int key0) {
 #pragma unroll
         for (int i = 0; i < NU; i++) {
             const int u = tid + kThreads * i;
             kid[i] = bt[chunk_block_of(a, min(key0 + u / (D / 16), key_end - 1))];
 #pragma unroll
-            for (int r = 0; r < (ALIGN4 ? 1 : 4); r++)
+            for (int r = 0; r < (PAGE4 ? 1 : 4); r++)
                 vid[i][r] = bt[chunk_block_of(a, min(key0 + 4 * (u / DW) + r, key_end - 1))];
         }
     };
@@ -287,7 +304,7 @@ __device__ __forceinline__ void chunk_attn_body(const ChunkArgs &a, int bid) {
             kreg[i] = u32x4{0, 0, 0, 0};
             if (kp < key_end) kreg[i] = *reinterpret_cast<const u32x4 *>(a.k_cache + row_of(kid[i], kp) * DW + 4 * c16);
             const int ddw = u % DW, vp = key0 + 4 * (u / DW);
-            if constexpr (ALIGN4) {
+            if constexpr (PAGE4) {
                 const uint32_t *vr = a.v_cache + row_of(vid[i][0], min(vp, key_end - 1) & ~3) * DW + ddw;
 #pragma unroll
                 for (int r = 0; r < 4; r++) vreg[i][r] = vp + r < key_end ? vr[r * DW] : 0u;
@@ -505,14 +522,16 @@ __device__ __forceinline__ void chunk_attn_body(const ChunkArgs &a, int bid) {
 }
 
 // ---- tiles through LDS on the 32x32 matrix instructions -----------------------------------------------------------------
-// The split and the numerics of chunk_attn_kernel, and the instruction mix of the prefill kernel's d = 64 form: vector
-// issue bounds this head dim, and an instruction of 32x32 holds it half as long per product as two of 16x16 --
+// The split and the numerics of chunk_attn_body, and the instruction mix of the prefill kernel's d = 64 form: vector
+// issue bounds these head dims, and an instruction of 32x32 holds it half as long per product as two of 16x16 --
 //     S^T[32 keys, 32 cols] = v_mfma_f32_32x32x64_f8f6f4 (E5M2 bytes as they are: the whole head dim) or four of
 //                             v_mfma_f32_32x32x16_f16 (E4M3, decoded);   O^T[32 dims, 32 cols] += v_mfma_f32_32x32x16_f16
 // A wave owns 32 * CB columns.  Lane l: n = l % 32 the column, h = l / 32; accumulator register r is row
 // 8 (r / 4) + 4 h + r % 4.  Registers 8 s .. 8 s + 7 of the scores are the k-slots of the second product's step s if V^T
 // holds the keys of every group of 16 in the order 0 1 2 3 8 9 10 11 | 4 5 6 7 12 13 14 15.
 // PAGE16 (block_size % 16 == 0): the 16 keys that a wave stages share a block, whose address is then scalar.
+// Against chunk_attn_body: d = 64, E5M2, the chunk of 2048 rows above 320 -> 155 us; d = 128, 512 rows over 4000 keys
+// 42 -> 33 us; d = 256 (4 waves of 32 columns, one wave per SIMD) 28 -> 48 us, so that one stays.
 typedef int int8p_t __attribute__((ext_vector_type(8)));
 
 template <int D, int MODE, int CB, int WAVES, bool PAGE16, bool ZS>
@@ -889,6 +908,10 @@ __device__ __forceinline__ void chunk_attn32_body(const ChunkArgs &a, int bid) {
 // only, which is what lets NB = 4 at D = 128 keep enough bytes in flight.
 // RING = 0 (any block size): rows go to registers, NF steps in flight, an address for every key.
 // Each wave keeps its own reference point and sums; they are joined through LDS, and the ranges by the merge kernel.
+// Measured: 16 rows of 32 heads on 8 at context 65537, d = 128, E4M3 47 + 6 us for 134 MB, 2.9 TB/s in the kernel (E5M2
+// 43 + 6 us); 32 requests with 3 to 8 rows, contexts to 4096, 32 heads on 4, d = 64, E4M3 24 + 5 us for 39 MB: a wave has
+// five steps there, and the round trips in front of them (lengths, block ids, rows), the exponentials of 64 columns and the
+// join bound it.  Registers instead of the ring (RING = 0 everywhere): 51 and 34 us.
 template <int D>
 struct NarrowStep {
     u32x4 kw[2][D / 64];
@@ -1334,15 +1357,24 @@ __device__ __forceinline__ void chunk_narrow_body(const ChunkArgs &a, int pair, 
 
 // ---- kernels: the LDS kernel alone, the narrow one alone, or both in one grid ------------------------------------------
 // Workgroup of the LDS kernels per head dim: columns, waves, keys per tile, and waves per SIMD that the registers are for.
+// The others measured (us, kernel alone; "2048 rows" is the chunk of the table at the top):
+//   d = 64:  256 columns, 4 waves 142; 256 in 8 waves 176; 512 in 8 waves 171 (2048 rows, E5M2)
+//   d = 128: 128 columns, 4 waves 243; 256 in 8 waves 231 + 18 of the merge that it then needs; 256 in 4 waves 258 (2048 rows, E5M2)
+//   d = 256: 128 columns, 8 waves 210 / 217; 128 in 4 waves 289 / 326; 256 in 8 waves 380 / 628, spills (2048 rows, E5M2 / E4M3)
+//   d = 512: 128 columns, 8 waves 425 / 543; 64 in 4 waves 901 / 1067; 128 in 4 waves 590 / 1465 (2048 rows, E5M2 / E4M3);
+//            3 x 150 rows over 1501 keys, E4M3: 85 with 128 columns, 85 with 64
 struct WideShape { int columns, waves, keys, occ; };
 constexpr int kMost32 = 128;             // largest head dim on the 32x32 instructions
 static constexpr WideShape wide_shape(int64_t d) {
     return d == 64 ? WideShape{256, 4, 64, 2} : (d == 128 ? WideShape{128, 4, 64, 2} : (d == 256 ? WideShape{128, 8, 64, 1} : WideShape{128, 8, 32, 1}));
 }
-// Steps in the ring of a wave of the narrow kernel (0: the rows go through registers).
+// Steps in the ring of a wave of the narrow kernel: what 160 KB of LDS hold beside the workgroups that the registers allow
+// (0: the rows go through registers; at d = 512 one step of four waves is 128 KB, and none would be in flight behind it).
 static constexpr int ring_steps(int d, int nb) { return d == 64 ? 4 : (d == 128 ? (nb == 4 ? 4 : 2) : (d == 256 ? 2 : 0)); }
 
-constexpr int mixed_blocks(int d) { return d <= 256 ? 2 : 1; }   // 16-column blocks of the narrow kernel beside the LDS kernel
+// 16-column blocks of the narrow kernel beside the LDS kernel.  Single rows need one (16 of them beside a chunk of 512
+// rows, d = 128: 40.5 us instead of 43.8); drafts beside a prompt need two, and would be mostly empty LDS tiles with one.
+constexpr int mixed_blocks(int d) { return d <= 256 ? 2 : 1; }
 constexpr size_t wide_lds(int d, int mode) {   // two (K, V^T) buffers; K rows of d bytes (E5M2) or halfs, 16 bytes more each
     const WideShape w = wide_shape(d);
     return (size_t)(w.keys * (mode == FEATHER_E5M2 ? d + 16 : 2 * d + 16) + 2 * d * w.keys) * 2;
@@ -1514,6 +1546,9 @@ struct ChunkPlan {
 static int log2_of(int64_t x) { int l = 0; while ((1ll << l) < x) l++; return l; }
 
 static int wide_columns(int64_t d) { return wide_shape(d).columns; }
+// Most 16-column blocks of the narrow kernel alone: what the registers hold.  64 columns against the LDS kernel (merge
+// included): 32 sequences of 4096 keys, d = 64, E4M3 36 us against 40; 4 of them 17 against 19; 2 of 400 keys 11.5 against
+// 16; 32 of 4096 keys, d = 128, E5M2 75 against 79.
 static int narrow_most_blocks(int64_t d) { return d <= 128 ? 4 : (d == 256 ? 2 : 1); }
 
 static int64_t chunk_slots(int64_t total_rows, int64_t n_seq, int64_t group, int qt) { return total_rows * group / qt + n_seq; }
@@ -1549,8 +1584,12 @@ static ChunkPlan chunk_plan(int64_t n_seq, int64_t total_rows, int64_t n_q_heads
     }
     p.narrow_rows = p.wide && p.narrow ? (int)(p.col_split / group) : 0;
     const int64_t each = n_seq > 0 ? (total_rows + n_seq - 1) / n_seq * group : 1;   // columns of a sequence of average length
+    // 512 workgroups, two per CU: a chunk of 2048 rows, d = 64, 143 + 11 us; 256: 197; 1024: 139 + 14.  16 single rows beside
+    // 512 rows, d = 128: 44 + 8 us; 256: 56 + 5; 1024: 54 + 13.
     p.z_wide = p.wide ? ranges_for(n_seq * ((each + wide_columns(d) - 1) / wide_columns(d)) * n_kv_heads, 512, max_ctx, kChunkMinKeys) : 1;
     // the chip holds 256 workgroups of a kernel that fills a CU's registers, two or three times as many of a smaller one
+    // (drafts of 32 requests, d = 64, 64 columns: 512 workgroups 24 us, 768 29, 384 28; 16 rows at context 65537, d = 128,
+    // 64 columns: 256 workgroups 47 us, 512 61)
     const int weight = (int)(d / 64) * p.nb;
     const int64_t groups = 256 * (weight <= 2 ? 3 : (weight <= 4 ? 2 : 1));
     const int64_t tiles = (p.wide ? n_seq : n_seq * ((each + 16 * p.nb - 1) / (16 * p.nb))) * n_kv_heads;

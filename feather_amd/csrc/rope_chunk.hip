@@ -6,8 +6,12 @@
 // 64 bits, and so is the product: far positions make thousands of turns, of which only the fraction counts (a 32-bit
 // product at position 10^5 is off by 2^-8 of a turn).  The fraction is exact to 2^-53 * turns; from there on 32 bits do.
 //
-// A streaming kernel: 4 (or 2) bytes in, 1 byte out per element.  The angles of a token are computed once and shared
-// by its heads through LDS; the elements are requested before the position is looked up, so the two chains overlap.
+// A streaming kernel, bound by its bytes: 4 (or 2) in, 1 out per element.  The angles of a token are computed once per
+// workgroup and shared by its heads through LDS; the elements are requested before the position is looked up, so the
+// two chains overlap.  9 ragged chunks (4505 rows of 48 heads, d = 128, fp32): 138 MB in 37 us, 3.7 TB/s of the 5.1 that
+// a copy reaches (27 us); one token for 32 requests (40 heads of 64): 3.7 us, three dependent memory round trips.  More
+// units per thread, so that fewer workgroups compute the angles: 2, 3 or 4 of them 41, 37 and 39 us, and 4.3, 4.5 and
+// 4.6 us for the single tokens -- not worth it.
 #include "common.h"
 
 namespace feather {
@@ -68,10 +72,10 @@ __device__ __forceinline__ float4_t rope_load4(const void *p, int64_t at) {
     }
 }
 
-// Workgroups [0, n_seq): one wave each answers for a sequence.  The others: `parts` workgroups per token, each with an
-// equal share of the token's units.  A unit is 4 + 4 elements: a pair group of the half layout (elements 4t .. and
-// their partners rot / 2 further on), or eight neighbours (interleaved pairs, dims that are not rotated, v).
-template <int MODE, bool F16, int U>
+// Workgroups [0, n_seq): one wave each answers for a sequence.  The others: `parts` workgroups per token, a unit per
+// thread.  A unit is 4 + 4 elements: a pair group of the half layout (elements 4t .. and their partners rot / 2 further
+// on), or eight neighbours (interleaved pairs, dims that are not rotated, v).
+template <int MODE, bool F16>
 __global__ __launch_bounds__(kRcThreads) void rope_chunk_kernel(RopeChunkArgs a, int parts) {
     __shared__ __attribute__((aligned(16))) float cs[2 * kRcMaxPairs];
     if ((int)blockIdx.x < a.n_seq) {
@@ -81,25 +85,14 @@ __global__ __launch_bounds__(kRcThreads) void rope_chunk_kernel(RopeChunkArgs a,
     const int item = blockIdx.x - a.n_seq;
     const int row = item / parts, part = item - row * parts;
     const int heads = a.n_q + 2 * a.n_kv, per_head = a.d / 8, units = heads * per_head;
-    const int half = a.rot / 2, rot_units = a.rot / 8;
-    const int64_t base = (int64_t)row * a.row_stride;
-    float4_t lo[U], hi[U];
-    int head[U], at_lo[U], at_hi[U], pair[U];
-    bool live[U];
-#pragma unroll
-    for (int i = 0; i < U; i++) {
-        const int u = (part * U + i) * kRcThreads + (int)threadIdx.x;
-        live[i] = u < units;
-        head[i] = live[i] ? u / per_head : 0;
-        const int t = live[i] ? u - head[i] * per_head : 0;
-        const bool turns = t < rot_units && head[i] < a.n_q + a.n_kv;
-        const bool split = turns && !a.interleaved;
-        at_lo[i] = split ? 4 * t : 8 * t;
-        at_hi[i] = split ? half + 4 * t : 8 * t + 4;
-        pair[i] = turns ? 4 * t : -1;
-        lo[i] = rope_load4<F16>(a.qkv, base + (int64_t)head[i] * a.d + at_lo[i]);
-        hi[i] = rope_load4<F16>(a.qkv, base + (int64_t)head[i] * a.d + at_hi[i]);
-    }
+    const int half = a.rot / 2;
+    const int u = part * kRcThreads + (int)threadIdx.x;
+    const bool live = u < units;
+    const int head = live ? u / per_head : 0, t = live ? u - head * per_head : 0;
+    const bool turns = t < a.rot / 8 && head < a.n_q + a.n_kv, split = turns && !a.interleaved;
+    const int at_lo = split ? 4 * t : 8 * t, at_hi = split ? half + 4 * t : 8 * t + 4;
+    const int64_t from = (int64_t)row * a.row_stride + (int64_t)head * a.d;
+    float4_t lo = rope_load4<F16>(a.qkv, from + at_lo), hi = rope_load4<F16>(a.qkv, from + at_hi);
     // ---- the row's sequence: the last one that starts at or before it (64 per step)
     int below = 0;
     for (int s0 = 0; s0 < a.n_seq; s0 += kWave) {
@@ -110,23 +103,17 @@ __global__ __launch_bounds__(kRcThreads) void rope_chunk_kernel(RopeChunkArgs a,
     }
     const int seq = __builtin_amdgcn_readfirstlane(below - 1);
     const bool inside = seq >= 0 && row < a.cu_seqlens[max(seq, 0) + 1];
+    float *const rot_out = a.rot_f32 ? a.rot_f32 + ((int64_t)row * heads + head) * a.d : nullptr;
     if (!inside) {                                    // a row of no sequence
-        if (a.fill) {
-#pragma unroll
-            for (int i = 0; i < U; i++)
-                if (live[i] && head[i] < a.n_q) {
-                    uint32_t *dst = a.q_packed + ((int64_t)row * a.n_q + head[i]) * (a.d / 4);
-                    dst[at_lo[i] / 4] = 0u;
-                    dst[at_hi[i] / 4] = 0u;
-                }
-            if (a.rot_f32) {
-#pragma unroll
-                for (int i = 0; i < U; i++)
-                    if (live[i]) {
-                        float *r = a.rot_f32 + ((int64_t)row * heads + head[i]) * a.d;
-                        *reinterpret_cast<float4_t *>(r + at_lo[i]) = float4_t{0.f, 0.f, 0.f, 0.f};
-                        *reinterpret_cast<float4_t *>(r + at_hi[i]) = float4_t{0.f, 0.f, 0.f, 0.f};
-                    }
+        if (a.fill && live) {
+            if (head < a.n_q) {
+                uint32_t *dst = a.q_packed + ((int64_t)row * a.n_q + head) * (a.d / 4);
+                dst[at_lo / 4] = 0u;
+                dst[at_hi / 4] = 0u;
+            }
+            if (rot_out) {
+                *reinterpret_cast<float4_t *>(rot_out + at_lo) = float4_t{0.f, 0.f, 0.f, 0.f};
+                *reinterpret_cast<float4_t *>(rot_out + at_hi) = float4_t{0.f, 0.f, 0.f, 0.f};
             }
         }
         return;
@@ -137,62 +124,57 @@ __global__ __launch_bounds__(kRcThreads) void rope_chunk_kernel(RopeChunkArgs a,
     int blk = -1;
     if (pos_ok) blk = a.block_tables[(int64_t)seq * a.max_blocks + entry];
     for (int j = threadIdx.x; j < half; j += kRcThreads) {
-        double t = (double)pos * a.freq[j];
-        t -= rint(t);                                 // fraction of a turn, [-1/2, 1/2]
-        const double k = rint(4.0 * t);
+        double x = (double)pos * a.freq[j];
+        x -= rint(x);                                 // fraction of a turn, [-1/2, 1/2]
+        const double k = rint(4.0 * x);
         float s, c;
-        sincos_quadrant((float)((t - 0.25 * k) * 6.283185307179586), (int)k, s, c);
+        sincos_quadrant((float)((x - 0.25 * k) * 6.283185307179586), (int)k, s, c);
         cs[2 * j] = c * a.amplitude;
         cs[2 * j + 1] = s * a.amplitude;
     }
     __syncthreads();
-    const bool append = (unsigned)blk < (unsigned)a.n_blocks;
-    const int64_t slot = append ? ((int64_t)blk * a.n_kv) * a.block_size + ((int)pos - entry * a.block_size) : 0;
+    if (!live) return;
+    if (turns) {
+        const float4_t p0 = *reinterpret_cast<const float4_t *>(&cs[8 * t]), p1 = *reinterpret_cast<const float4_t *>(&cs[8 * t + 4]);
+        const float c[4] = {p0[0], p0[2], p1[0], p1[2]}, s[4] = {p0[1], p0[3], p1[1], p1[3]};
+        if (!a.interleaved) {
 #pragma unroll
-    for (int i = 0; i < U; i++) {
-        if (!live[i]) continue;
-        if (pair[i] >= 0) {
-            const float4_t p0 = *reinterpret_cast<const float4_t *>(&cs[2 * pair[i]]), p1 = *reinterpret_cast<const float4_t *>(&cs[2 * pair[i] + 4]);
-            const float c[4] = {p0[0], p0[2], p1[0], p1[2]}, s[4] = {p0[1], p0[3], p1[1], p1[3]};
-            if (!a.interleaved) {
+            for (int e = 0; e < 4; e++) {
+                const float x = lo[e], y = hi[e];
+                lo[e] = x * c[e] - y * s[e];
+                hi[e] = y * c[e] + x * s[e];
+            }
+        } else {
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float x = lo[i][e], y = hi[i][e];
-                    lo[i][e] = x * c[e] - y * s[e];
-                    hi[i][e] = y * c[e] + x * s[e];
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const float x = lo[i][2 * e], y = lo[i][2 * e + 1], z = hi[i][2 * e], w = hi[i][2 * e + 1];
-                    lo[i][2 * e] = x * c[e] - y * s[e];
-                    lo[i][2 * e + 1] = y * c[e] + x * s[e];
-                    hi[i][2 * e] = z * c[2 + e] - w * s[2 + e];
-                    hi[i][2 * e + 1] = w * c[2 + e] + z * s[2 + e];
-                }
+            for (int e = 0; e < 2; e++) {
+                const float x = lo[2 * e], y = lo[2 * e + 1], z = hi[2 * e], w = hi[2 * e + 1];
+                lo[2 * e] = x * c[e] - y * s[e];
+                lo[2 * e + 1] = y * c[e] + x * s[e];
+                hi[2 * e] = z * c[2 + e] - w * s[2 + e];
+                hi[2 * e + 1] = w * c[2 + e] + z * s[2 + e];
             }
         }
-        if (a.rot_f32) {                              // the values the codes are rounded from
-            float *r = a.rot_f32 + ((int64_t)row * heads + head[i]) * a.d;
-            *reinterpret_cast<float4_t *>(r + at_lo[i]) = lo[i];
-            *reinterpret_cast<float4_t *>(r + at_hi[i]) = hi[i];
-        }
-        uint32_t *dst;
-        if (head[i] < a.n_q) {
-            dst = a.q_packed + ((int64_t)row * a.n_q + head[i]) * (a.d / 4);
-        } else {
-            if (!append) continue;
-            const bool is_k = head[i] < a.n_q + a.n_kv;
-            const int kvh = head[i] - a.n_q - (is_k ? 0 : a.n_kv);
-            dst = (is_k ? a.k_cache : a.v_cache) + (slot + (int64_t)kvh * a.block_size) * (a.d / 4);
-        }
-        const uint32_t wlo = quant4<MODE>(lo[i][0], lo[i][1], lo[i][2], lo[i][3]), whi = quant4<MODE>(hi[i][0], hi[i][1], hi[i][2], hi[i][3]);
-        if (at_hi[i] == at_lo[i] + 4) {               // neighbours (8 bytes from a multiple of 8 on: d is one)
-            *reinterpret_cast<u32x2 *>(dst + at_lo[i] / 4) = u32x2{wlo, whi};
-        } else {
-            dst[at_lo[i] / 4] = wlo;
-            dst[at_hi[i] / 4] = whi;
-        }
+    }
+    if (rot_out) {                                    // the values the codes are rounded from
+        *reinterpret_cast<float4_t *>(rot_out + at_lo) = lo;
+        *reinterpret_cast<float4_t *>(rot_out + at_hi) = hi;
+    }
+    uint32_t *dst;
+    if (head < a.n_q) {
+        dst = a.q_packed + ((int64_t)row * a.n_q + head) * (a.d / 4);
+    } else {
+        if ((unsigned)blk >= (unsigned)a.n_blocks) return;
+        const bool is_k = head < a.n_q + a.n_kv;
+        const int kvh = head - a.n_q - (is_k ? 0 : a.n_kv);
+        const int64_t slot = ((int64_t)blk * a.n_kv + kvh) * a.block_size + ((int)pos - entry * a.block_size);
+        dst = (is_k ? a.k_cache : a.v_cache) + slot * (a.d / 4);
+    }
+    const uint32_t wlo = quant4<MODE>(lo[0], lo[1], lo[2], lo[3]), whi = quant4<MODE>(hi[0], hi[1], hi[2], hi[3]);
+    if (!split) {                                     // neighbours (8 bytes from a multiple of 8 on: d is one)
+        *reinterpret_cast<u32x2 *>(dst + at_lo / 4) = u32x2{wlo, whi};
+    } else {
+        dst[at_lo / 4] = wlo;
+        dst[at_hi / 4] = whi;
     }
 }
 
@@ -240,22 +222,13 @@ extern "C" int feather_rope_append_chunk(const void *qkv, int src_f16, int64_t r
     a.block_size = (int)block_size; a.max_blocks = (int)max_blocks; a.n_blocks = (int)n_blocks;
     a.interleaved = layout == FEATHER_ROPE_INTERLEAVED; a.fill = fill; a.amplitude = amplitude;
     const int64_t units = heads * (d / 8);
-    const int U = units <= kRcThreads ? 1 : (units <= 2 * kRcThreads ? 2 : (units <= 3 * kRcThreads ? 3 : 4));
-    const int64_t parts = (units + U * kRcThreads - 1) / (U * kRcThreads);
+    const int64_t parts = (units + kRcThreads - 1) / kRcThreads;
     const int64_t grid = n_seq + total_rows * parts;
     FEATHER_CHECK(grid < (1ll << 31), FEATHER_ESHAPE, "%s: grid too large", me);
-#define FEATHER_RC(MM, FF, UU)                                                                                         \
-    hipLaunchKernelGGL((rope_chunk_kernel<MM, FF, UU>), dim3((unsigned)grid), dim3(kRcThreads), 0, (hipStream_t)stream, a, (int)parts)
-#define FEATHER_RCU(MM, FF)                                                                                            \
-    do {                                                                                                               \
-        if (U == 1) FEATHER_RC(MM, FF, 1);                                                                             \
-        else if (U == 2) FEATHER_RC(MM, FF, 2);                                                                        \
-        else if (U == 3) FEATHER_RC(MM, FF, 3);                                                                        \
-        else FEATHER_RC(MM, FF, 4);                                                                                    \
-    } while (0)
-    if (mode == FEATHER_E5M2) { if (src_f16) FEATHER_RCU(FEATHER_E5M2, true); else FEATHER_RCU(FEATHER_E5M2, false); }
-    else { if (src_f16) FEATHER_RCU(FEATHER_E4M3, true); else FEATHER_RCU(FEATHER_E4M3, false); }
-#undef FEATHER_RCU
+#define FEATHER_RC(MM, FF)                                                                                             \
+    hipLaunchKernelGGL((rope_chunk_kernel<MM, FF>), dim3((unsigned)grid), dim3(kRcThreads), 0, (hipStream_t)stream, a, (int)parts)
+    if (mode == FEATHER_E5M2) { if (src_f16) FEATHER_RC(FEATHER_E5M2, true); else FEATHER_RC(FEATHER_E5M2, false); }
+    else { if (src_f16) FEATHER_RC(FEATHER_E4M3, true); else FEATHER_RC(FEATHER_E4M3, false); }
 #undef FEATHER_RC
     return check_launch(me);
 }
