@@ -8,7 +8,7 @@ tables, lengths and counts; the caches are updated in place, in blocks that were
 """
 from __future__ import annotations
 
-import ctypes
+import array
 import operator
 
 import torch
@@ -30,7 +30,7 @@ _dtype, _shape = operator.attrgetter("dtype"), operator.attrgetter("shape")
 
 
 def _pool(caches, ref_counts: torch.Tensor):
-    """Checks the caches against the pool; returns their pointers as a C array, how many, and the bytes and tokens of a
+    """Checks the caches against the pool; returns their pointers as an array, how many, and the bytes and tokens of a
     block.  (A decoder has dozens of caches: every check is one pass in C over all of them.)"""
     caches = tuple(caches)
     if not caches:
@@ -58,7 +58,7 @@ def _pool(caches, ref_counts: torch.Tensor):
         raise ValueError(f"ref_counts must be [n_blocks={n_blocks}] with at least one block")
     if ref_counts.device != first.device:
         raise ValueError("ref_counts and the caches must be on the same device")
-    return (ctypes.c_void_p * len(ptrs))(*ptrs), len(ptrs), block_bytes, block_size
+    return array.array("Q", ptrs), len(ptrs), block_bytes, block_size
 
 
 def paged_cache_fork(caches, block_tables: torch.Tensor, ctx_lens: torch.Tensor, ref_counts: torch.Tensor,
@@ -89,7 +89,7 @@ def paged_cache_fork(caches, block_tables: torch.Tensor, ctx_lens: torch.Tensor,
     tables_out, ctx_out, ref_out = torch.empty_like(block_tables), torch.empty_like(ctx_lens), torch.empty_like(ref_counts)
     status = torch.empty_like(ctx_lens)
     scratch = ref_counts.new_empty(N.lib().feather_paged_cache_fork_scratch_bytes(n_seq, n_blocks) // 4)
-    N.call(dev, "feather_paged_cache_fork", ctypes.addressof(ptrs), n_caches, block_bytes, block_tables.data_ptr(),
+    N.call(dev, "feather_paged_cache_fork", ptrs.buffer_info()[0], n_caches, block_bytes, block_tables.data_ptr(),
            ctx_lens.data_ptr(), ref_counts.data_ptr(), parents.data_ptr(), room.data_ptr() if room is not None else None,
            tables_out.data_ptr(), ctx_out.data_ptr(), ref_out.data_ptr(), status.data_ptr(), scratch.data_ptr(), n_seq, max_blocks,
            block_size, n_blocks)
@@ -112,7 +112,7 @@ def paged_cache_compact(caches, block_tables: torch.Tensor, ref_counts: torch.Te
     tables_out, ref_out, block_map = torch.empty_like(block_tables), torch.empty_like(ref_counts), torch.empty_like(ref_counts)
     n_live = ref_counts.new_empty(1)
     scratch = ref_counts.new_empty(N.lib().feather_paged_cache_compact_scratch_bytes(n_blocks) // 4)
-    N.call(dev, "feather_paged_cache_compact", ctypes.addressof(ptrs), n_caches, block_bytes, block_tables.data_ptr(),
+    N.call(dev, "feather_paged_cache_compact", ptrs.buffer_info()[0], n_caches, block_bytes, block_tables.data_ptr(),
            ref_counts.data_ptr(), tables_out.data_ptr(), ref_out.data_ptr(), block_map.data_ptr(), n_live.data_ptr(), scratch.data_ptr(),
            block_tables.numel(), n_blocks)
     return tables_out, ref_out, block_map, n_live
