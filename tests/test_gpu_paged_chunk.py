@@ -123,6 +123,8 @@ SHAPES = [
     ([65], [257], 3, 1, 256, 6),
     ([7, 20], [7, 130], 4, 2, 512, 16),
     ([40], [290], 2, 1, 512, 7),
+    ([150, 3], [400, 70], 2, 1, 512, 16),                 # several tiles at the widest head
+    ([210, 64], [1203, 65], 4, 2, 256, 16),
     ([4], [2049], 16, 1, 64, 16),                         # few columns, a long cache: ranges
     ([1, 1, 1], [3000, 1, 777], 8, 1, 128, 16),
 ]
@@ -329,3 +331,12 @@ def test_out_that_overlaps_an_input_is_refused():
     with pytest.raises(ValueError, match="overlaps"):
         paged_chunk_attention_fp8_acc_fp32_gpu(q, kc, kc.clone(), tables, cu, ctx, out_dtype=torch.uint32,
                                                out=kc.view(-1)[64:256].view(3, 64).view(torch.uint32))
+
+
+@pytest.mark.parametrize("lens,ctx,Hq,Hkv,d", [([1, 7, 3], [2900, 611, 1500], 8, 2, 64), ([300, 1, 1], [900, 2000, 33], 8, 2, 128),
+                                               ([150, 2], [1500, 900], 4, 4, 256), ([140], [777], 2, 1, 512)])
+def test_results_do_not_change_from_call_to_call(dev, orc, lens, ctx, Hq, Hkv, d):
+    P = _problem(orc, 9, lens, ctx, Hq, Hkv, d, 16, "E4M3")
+    first = _call(P, dev, True)
+    for _ in range(5):
+        assert torch.equal(_call(P, dev, True).view(torch.int32), first.view(torch.int32))
