@@ -50,6 +50,7 @@ struct ChunkArgs {
     int causal, out_kind, fill;
     int z_wide, z_narrow;             // most key ranges of a tile in either kernel
     float per_group;                  // KV heads over the workgroups of the narrow kernel that the chip holds at once
+    int narrow_tiles;                 // tiles of a sequence in the narrow kernel, if its rows are bounded as the caller says
     int narrow_rows;                  // beside the LDS kernel: rows a sequence of the narrow one can have (0: it runs alone)
     float *part_narrow;               // its partial results, then the (maximum, sum) pairs, then the keys per range
     int col_split;                    // sequences of more columns than this take the LDS kernel, the others the narrow one
@@ -895,8 +896,8 @@ __device__ __forceinline__ void chunk_attn32_body(const ChunkArgs &a, int bid) {
 }
 
 // ---- few columns: keys straight from the cache ----------------------------------------------------------------------
-// A drafted token or a handful of them: 16 * NB columns or fewer per (sequence, KV head), so the cache is read once and
-// its bytes bound the kernel.  One workgroup of four waves per (tile, KV head, key range); the waves take the range's
+// A drafted token or a handful of them: few tiles of 16 * NB columns per (sequence, KV head), so the cache is read once or a
+// few times and its bytes bound the kernel.  One workgroup of four waves per (tile, KV head, key range); the waves take the range's
 // steps of 32 keys in turn and share nothing until the end:
 //     S^T[key, col]   = K Q^T       a lane holds 16 codes of one key: the A operand of two products
 //     O_c^T[i, col]  += V_c^T P^T   dim = 4 i + c: the lane holds the same word of eight keys and byte c of them is the
@@ -905,11 +906,11 @@ __device__ __forceinline__ void chunk_attn32_body(const ChunkArgs &a, int bid) {
 // memory to LDS without passing through registers, RING steps of a wave in flight or in use, into a ring of the wave's
 // own (no barrier, only the wave's count of outstanding loads).  A load moves 1 KiB with a wave-uniform base -- the block
 // id is a scalar load, the address scalar arithmetic -- and the lane's constant offset.  Registers then hold one step
-// only, which is what lets NB = 4 at D = 128 keep enough bytes in flight.
+// only.
 // RING = 0 (any block size): rows go to registers, NF steps in flight, an address for every key.
 // Each wave keeps its own reference point and sums; they are joined through LDS, and the ranges by the merge kernel.
 // Measured: 16 rows of 32 heads on 8 at context 65537, d = 128, E4M3 47 + 6 us for 134 MB, 2.9 TB/s in the kernel (E5M2
-// 43 + 6 us); 32 requests with 3 to 8 rows, contexts to 4096, 32 heads on 4, d = 64, E4M3 24 + 5 us for 39 MB: a wave has
+// 39 + 6 us); 32 requests with 3 to 8 rows, contexts to 4096, 32 heads on 4, d = 64, E4M3 24 + 5 us for 39 MB: a wave has
 // five steps there, and the round trips in front of them (lengths, block ids, rows), the exponentials of 64 columns and the
 // join bound it.  Registers instead of the ring (RING = 0 everywhere): 51 and 34 us.
 template <int D>
@@ -958,7 +959,7 @@ __device__ __forceinline__ int64_t narrow_item(const ChunkArgs &a, int64_t item,
 }
 
 template <int D, int MODE, int NB, int RING>
-__device__ __forceinline__ void chunk_narrow_body(const ChunkArgs &a, int pair, int zr) {
+__device__ __forceinline__ void chunk_narrow_body(const ChunkArgs &a, int pair, int tile, int zr) {
     constexpr int DW = D / 4, RB = D / 64, STEPS = D / 32, QT = 16 * NB, W = 4, STEP = 32;
     constexpr bool BF8 = MODE == FEATHER_E5M2;
     constexpr int NF = RING > 0 ? 1 : (D == 64 ? (NB == 4 ? 2 : 4) : (D == 128 ? 2 : 1));
@@ -968,8 +969,8 @@ __device__ __forceinline__ void chunk_narrow_body(const ChunkArgs &a, int pair, 
     float4_t *const x_lds = reinterpret_cast<float4_t *>(smem);     // [NB][W][RB * 4][64]
 
     // In launch order, which goes round the XCDs, all first ranges come before all second ones and so on: ranges that do
-    // not exist come last.  A sequence has one tile here -- unless the caller's bound of its rows was wrong, then the
-    // workgroup takes its tiles one after the other.
+    // not exist come last.  A workgroup has one tile of its sequence -- unless the caller's bound of the rows was wrong, then
+    // it takes others after it.
     const int seq_i = (int)(__umulhi(2u * (uint32_t)pair, a.kv_mul) >> a.kv_shift), kvh = pair - seq_i * a.n_kv_heads;
     ChunkTile t;
     t.seq = seq_i;
@@ -980,11 +981,11 @@ __device__ __forceinline__ void chunk_narrow_body(const ChunkArgs &a, int pair, 
     int least = kNarrowMinKeys;
     if (a.z_narrow > 1) {
         least = narrow_min_keys(a, QT);
-        if (pair + zr == 0 && threadIdx.x == 0) *reinterpret_cast<int *>(a.part_narrow + narrow_items(a) * a.z_narrow * (D + 2)) = least;
+        if (pair + tile + zr == 0 && threadIdx.x == 0) *reinterpret_cast<int *>(a.part_narrow + narrow_items(a) * a.z_narrow * (D + 2)) = least;
     }
     if (t.cols > a.col_split) return;                               // a long run of rows: the other kernel's work
 #pragma nounroll
-    for (int col0 = 0; col0 < t.cols; col0 += QT) {
+    for (int col0 = tile * QT; col0 < t.cols; col0 += a.narrow_tiles * QT) {
     chunk_tile_at(a, col0, QT, t);
     const int per = chunk_range_keys(t.keys, a.z_narrow, kNarrowStep, least);
     const int key_begin = zr * per, key_end = min(t.keys, key_begin + per);
@@ -1351,7 +1352,7 @@ __device__ __forceinline__ void chunk_narrow_body(const ChunkArgs &a, int pair, 
     }
     if (a.z_narrow > 1 && u0 == 0 && kb == 0) *reinterpret_cast<float2p_t *>(a.part_narrow + a.z_narrow * items * D + at * 2) = float2p_t{m, sum};
     }
-    if (t.cols > QT) __syncthreads();                                // the next tile writes the exchange area
+    if (t.cols > a.narrow_tiles * QT) __syncthreads();               // the next tile writes the exchange area
     }
 }
 
@@ -1368,9 +1369,9 @@ constexpr int kMost32 = 128;             // largest head dim on the 32x32 instru
 static constexpr WideShape wide_shape(int64_t d) {
     return d == 64 ? WideShape{256, 4, 64, 2} : (d == 128 ? WideShape{128, 4, 64, 2} : (d == 256 ? WideShape{128, 8, 64, 1} : WideShape{128, 8, 32, 1}));
 }
-// Steps in the ring of a wave of the narrow kernel: what 160 KB of LDS hold beside the workgroups that the registers allow
+// Steps in the ring of a wave of the narrow kernel: what 160 KB of LDS hold with the workgroups that the registers allow
 // (0: the rows go through registers; at d = 512 one step of four waves is 128 KB, and none would be in flight behind it).
-static constexpr int ring_steps(int d, int nb) { return d == 64 ? 4 : (d == 128 ? (nb == 4 ? 4 : 2) : (d == 256 ? 2 : 0)); }
+static constexpr int ring_steps(int d, int nb) { return d == 64 ? 4 : (d <= 256 ? 2 : 0); }
 
 // 16-column blocks of the narrow kernel beside the LDS kernel.  Single rows need one (16 of them beside a chunk of 512
 // rows, d = 128: 40.5 us instead of 43.8); drafts beside a prompt need two, and would be mostly empty LDS tiles with one.
@@ -1401,7 +1402,8 @@ __global__ __launch_bounds__(64 * wide_shape(D).waves, wide_shape(D).occ) void c
 template <int D, int MODE, int NB, int RING>
 __global__ __launch_bounds__(256, (D / 64) * NB <= 4 ? 2 : 1) void chunk_narrow_kernel(ChunkArgs a, int fill) {
     if (fill && blockIdx.y == 0) chunk_fill_outside<D>(a, blockIdx.x, gridDim.x, 256);
-    if (a.n_seq > 0) chunk_narrow_body<D, MODE, NB, RING>(a, blockIdx.x, blockIdx.y);
+    const int pairs = a.n_seq * a.n_kv_heads, tile = pairs > 0 ? blockIdx.x / pairs : 0;
+    if (a.n_seq > 0) chunk_narrow_body<D, MODE, NB, RING>(a, blockIdx.x - tile * pairs, tile, blockIdx.y);
 }
 
 // A batch of long and short runs of rows: the tiles first, whose matrix work then shares the CUs with the streaming of the
@@ -1418,7 +1420,7 @@ __global__ __launch_bounds__(256, wide_shape(D).occ) void chunk_mixed_kernel(Chu
     bid -= wide;
     if (bid < narrow) {
         const int zr = bid / pairs;
-        chunk_narrow_body<D, MODE, NB, PAGE16 ? ring_steps(D, NB) : 0>(a, bid - zr * pairs, zr);
+        chunk_narrow_body<D, MODE, NB, PAGE16 ? ring_steps(D, NB) : 0>(a, bid - zr * pairs, 0, zr);
     } else {
         chunk_fill_outside<D>(a, bid - narrow, gridDim.x - wide - narrow, 256);
     }
@@ -1536,7 +1538,7 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(ChunkArgs a, int qt_wi
 // How a call is cut: which kernels run, their tiles, and into how many key ranges.
 struct ChunkPlan {
     bool wide, narrow;
-    int nb;                 // 16-column blocks of a narrow tile
+    int nb, tiles;          // 16-column blocks of a narrow tile; tiles of a sequence
     int col_split;
     int z_wide, z_narrow, narrow_rows;
     float per_group;
@@ -1546,10 +1548,19 @@ struct ChunkPlan {
 static int log2_of(int64_t x) { int l = 0; while ((1ll << l) < x) l++; return l; }
 
 static int wide_columns(int64_t d) { return wide_shape(d).columns; }
-// Most 16-column blocks of the narrow kernel alone: what the registers hold.  64 columns against the LDS kernel (merge
-// included): 32 sequences of 4096 keys, d = 64, E4M3 36 us against 40; 4 of them 17 against 19; 2 of 400 keys 11.5 against
-// 16; 32 of 4096 keys, d = 128, E5M2 75 against 79.
-static int narrow_most_blocks(int64_t d) { return d <= 128 ? 4 : (d == 256 ? 2 : 1); }
+// Most 16-column blocks of a tile of the narrow kernel: the accumulators and queries of two waves per SIMD (one at d = 256
+// and 512).  d = 128 with four blocks, one wave per SIMD: 32 sequences of 4096 keys, 64 columns, E5M2 74 us instead of 64.
+static constexpr int narrow_blocks(int64_t d) { return d == 64 ? 4 : (d <= 256 ? 2 : 1); }
+
+// Sequences of at most so many columns (in several tiles then, next to each other on an XCD) take the narrow kernel.  It
+// decodes for its own wave what the LDS kernel decodes once for a workgroup, and needs neither its barriers nor as many key
+// ranges.  LDS kernel against narrow kernel, us with the merge, n sequences of 4096 keys:
+//   d = 64:  256 columns 100 / 68 (n = 32, E4M3), 27 / 22 (4, E5M2); 512: 150 / 130 (32, E4M3), 31 / 29 (4, E5M2); 1024: 241 / 247
+//            (32, E4M3), 38 / 45 (4, E5M2)
+//   d = 128: 128 columns 143 / 121 (32, E5M2), 32 / 37 (4, E4M3); 256: 249 / 271 (32, E5M2), 42 / 57 (4, E4M3)
+//   d = 256: 64 columns 47 / 42 (4 of 8192, E4M3), 74 / 73 (16, E5M2); 128: 63 / 70, 95 / 70
+//   d = 512: 32 columns 50 / 41 (4 of 8192, E4M3), 74 / 59 (16, E5M2); 64: 55 / 65, 85 / 135
+static int narrow_columns(int64_t d) { return d == 64 ? 512 : (d == 128 ? 128 : (d == 256 ? 64 : 32)); }
 
 static int64_t chunk_slots(int64_t total_rows, int64_t n_seq, int64_t group, int qt) { return total_rows * group / qt + n_seq; }
 
@@ -1565,17 +1576,24 @@ static ChunkPlan chunk_plan(int64_t n_seq, int64_t total_rows, int64_t n_q_heads
                             int64_t max_q_len) {
     ChunkPlan p;
     const int64_t group = n_q_heads / n_kv_heads;
-    const int most = 16 * narrow_most_blocks(d);
     const int64_t rows_most = max_q_len > 0 && max_q_len < total_rows ? max_q_len : total_rows;   // rows of the longest sequence, if the hint is right
     const int64_t cols = rows_most * group;
-    if (cols <= most) {                 // all sequences are short (or the hint is wrong: more tiles each)
+    if (cols <= narrow_columns(d)) {    // all sequences are short (or the hint is wrong: more tiles each)
         p.narrow = true;
         p.wide = false;
         p.col_split = kAnyColumns;
-        p.nb = cols <= 16 ? 1 : (cols <= 32 ? 2 : 4);
+        const int64_t apart = n_seq * n_kv_heads * ranges_for(1, 128, max_ctx, kNarrowMinKeys);   // workgroups, at most, before columns are cut
+        auto tiles = [&](int nb) { return cols > 16 * nb ? (cols + 16 * nb - 1) / (16 * nb) : 1; };
+        // Tiles as wide as they get read the cache once; narrow ones are more workgroups, where a short context allows no
+        // ranges: two requests of 300 keys and 40 columns 9.9 us in one tile each, 6.3 in three; 32 requests of up to 4096 keys
+        // 24 us with 64 columns, 29 with 32, 32 with 16.
+        p.nb = 1;
+        while (p.nb < narrow_blocks(d) && tiles(p.nb) > 1 && apart * tiles(p.nb) > 256) p.nb *= 2;
+        p.tiles = (int)tiles(p.nb);
     } else {
         p.wide = true;
         p.nb = mixed_blocks((int)d);
+        p.tiles = 1;
         // with n_seq - 1 sequences of the longest length, can the last one be short?  (If the hint is wrong the LDS kernel
         // takes the short ones too.)
         const int64_t least = total_rows - (n_seq - 1) * rows_most;
@@ -1588,8 +1606,7 @@ static ChunkPlan chunk_plan(int64_t n_seq, int64_t total_rows, int64_t n_q_heads
     // 512 rows, d = 128: 44 + 8 us; 256: 56 + 5; 1024: 54 + 13.
     p.z_wide = p.wide ? ranges_for(n_seq * ((each + wide_columns(d) - 1) / wide_columns(d)) * n_kv_heads, 512, max_ctx, kChunkMinKeys) : 1;
     // the chip holds 256 workgroups of a kernel that fills a CU's registers, two or three times as many of a smaller one
-    // (drafts of 32 requests, d = 64, 64 columns: 512 workgroups 24 us, 768 29, 384 28; 16 rows at context 65537, d = 128,
-    // 64 columns: 256 workgroups 47 us, 512 61)
+    // (drafts of 32 requests, d = 64, 64 columns: 512 workgroups 24 us, 768 29, 384 28)
     const int weight = (int)(d / 64) * p.nb;
     const int64_t groups = 256 * (weight <= 2 ? 3 : (weight <= 4 ? 2 : 1));
     const int64_t tiles = (p.wide ? n_seq : n_seq * ((each + 16 * p.nb - 1) / (16 * p.nb))) * n_kv_heads;
@@ -1615,7 +1632,7 @@ static int launch_chunk_kernel(Kernel kern, dim3 grid, int threads, size_t lds, 
 
 template <int D, int MODE, int NB, int RING>
 static int launch_chunk_narrow(const ChunkArgs &a, bool fill, hipStream_t s) {
-    const int64_t pairs = a.n_seq > 0 ? (int64_t)a.n_seq * a.n_kv_heads : kChunkFillGroups;
+    const int64_t pairs = a.n_seq > 0 ? (int64_t)a.n_seq * a.n_kv_heads * a.narrow_tiles : kChunkFillGroups;
     FEATHER_CHECK(pairs * a.z_narrow < (1ll << 31), FEATHER_ESHAPE, "feather_paged_chunk_attn_fp8: grid too large");
     static unsigned long long lds_raised = 0;
     return launch_chunk_kernel(chunk_narrow_kernel<D, MODE, NB, RING>, dim3((unsigned)pairs, (unsigned)a.z_narrow), 256, narrow_lds(D, NB, RING), s, a,
@@ -1654,7 +1671,7 @@ static int launch_chunk(const ChunkArgs &a, const ChunkPlan &p, hipStream_t s) {
         if (p.nb == 1) rc = launch_chunk_narrow<D, MODE, 1, PAGE16 ? ring_steps(D, 1) : 0>(a, fill, s);
         if constexpr (D <= 256)
             if (p.nb == 2) rc = launch_chunk_narrow<D, MODE, 2, PAGE16 ? ring_steps(D, 2) : 0>(a, fill, s);
-        if constexpr (D <= 128)
+        if constexpr (D == 64)
             if (p.nb == 4) rc = launch_chunk_narrow<D, MODE, 4, PAGE16 ? ring_steps(D, 4) : 0>(a, fill, s);
     }
     if (rc != FEATHER_OK || !merge) return rc;
@@ -1747,7 +1764,7 @@ extern "C" int feather_paged_chunk_attn_fp8(const void *q, const void *k_cache, 
     a.group = (int)(n_q_heads / n_kv_heads); a.block_size = (int)block_size; a.max_blocks = (int)max_blocks;
     a.max_blk = (uint32_t)(n_blocks - 1);
     a.causal = causal; a.out_kind = out_kind; a.fill = fill;
-    a.z_wide = p.z_wide; a.z_narrow = p.z_narrow; a.per_group = p.per_group; a.narrow_rows = p.narrow_rows;
+    a.z_wide = p.z_wide; a.z_narrow = p.z_narrow; a.per_group = p.per_group; a.narrow_rows = p.narrow_rows; a.narrow_tiles = p.tiles;
     a.part_narrow = reinterpret_cast<float *>(static_cast<char *>(scratch) + chunk_wide_scratch(p)); a.col_split = p.col_split;
     a.scale_log2e = scale * 1.4426950408889634f;
     hipStream_t s = (hipStream_t)stream;

@@ -125,6 +125,11 @@ SHAPES = [
     ([40], [290], 2, 1, 512, 7),
     ([150, 3], [400, 70], 2, 1, 512, 16),                 # several tiles at the widest head
     ([210, 64], [1203, 65], 4, 2, 256, 16),
+    ([41], [700], 8, 1, 64, 16),                          # few columns, more than one tile of them
+    ([9, 64, 1], [9, 2050, 1100], 8, 1, 64, 12),
+    ([25], [900], 4, 1, 128, 16),
+    ([15], [600], 4, 1, 256, 16),
+    ([9], [700], 3, 1, 512, 16),
     ([4], [2049], 16, 1, 64, 16),                         # few columns, a long cache: ranges
     ([1, 1, 1], [3000, 1, 777], 8, 1, 128, 16),
 ]
