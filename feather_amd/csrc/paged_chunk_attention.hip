@@ -1361,7 +1361,8 @@ __device__ __forceinline__ void chunk_narrow_body(const ChunkArgs &a, int pair, 
 // The others measured (us, kernel alone; "2048 rows" is the chunk of the table at the top):
 //   d = 64:  256 columns, 4 waves 142; 256 in 8 waves 176; 512 in 8 waves 171 (2048 rows, E5M2)
 //   d = 128: 128 columns, 4 waves 243; 256 in 8 waves 231 + 18 of the merge that it then needs; 256 in 4 waves 258 (2048 rows, E5M2)
-//   d = 256: 128 columns, 8 waves 210 / 217; 128 in 4 waves 289 / 326; 256 in 8 waves 380 / 628, spills (2048 rows, E5M2 / E4M3)
+//   d = 256: 128 columns, 8 waves 210 / 217; 128 in 4 waves 289 / 326; 256 in 8 waves 380 / 628, spills; tiles of 32 keys 233 /
+//            236; 64 columns in 4 waves, 32 keys, two workgroups per CU 285 / 300 (2048 rows, E5M2 / E4M3)
 //   d = 512: 128 columns, 8 waves 425 / 543; 64 in 4 waves 901 / 1067; 128 in 4 waves 590 / 1465 (2048 rows, E5M2 / E4M3);
 //            3 x 150 rows over 1501 keys, E4M3: 85 with 128 columns, 85 with 64
 struct WideShape { int columns, waves, keys, occ; };
