@@ -977,6 +977,7 @@ __device__ __forceinline__ void chunk_narrow_body(const ChunkArgs &a, int pair, 
     t.row0 = chunk_clamp_row(a.cu_seqlens[seq_i], a.total_rows);
     t.rows = max(chunk_clamp_row(a.cu_seqlens[seq_i + 1], a.total_rows) - t.row0, 0);
     t.cols = t.rows * a.group;
+    if (tile > 0 && tile * QT >= t.cols) return;
     t.ctx = min(max(a.ctx_lens[seq_i], 0), a.max_blocks * a.block_size);
     int least = kNarrowMinKeys;
     if (a.z_narrow > 1) {
@@ -1377,6 +1378,11 @@ static constexpr int ring_steps(int d, int nb) { return d == 64 ? 4 : (d <= 256 
 // 16-column blocks of the narrow kernel beside the LDS kernel.  Single rows need one (16 of them beside a chunk of 512
 // rows, d = 128: 40.5 us instead of 43.8); drafts beside a prompt need two, and would be mostly empty LDS tiles with one.
 constexpr int mixed_blocks(int d) { return d <= 256 ? 2 : 1; }
+// Tiles of a sequence there (d = 64, 128: one grid with the LDS kernel, whose tiles would be mostly empty for drafts; the
+// second ones come last in it and mostly end at once).  16 sequences of 4000 keys beside a chunk of 512 rows: 10 rows of 4
+// heads, d = 128, E5M2 117 us with one tile (such sequences are the LDS kernel's then), 66 with two; 5 rows of 8 heads,
+// d = 64, E4M3 42 and 37; d = 256, two launches, 63 and 66.
+constexpr int mixed_tiles(int d) { return d <= 128 ? 2 : 1; }
 constexpr size_t wide_lds(int d, int mode) {   // two (K, V^T) buffers; K rows of d bytes (E5M2) or halfs, 16 bytes more each
     const WideShape w = wide_shape(d);
     return (size_t)(w.keys * (mode == FEATHER_E5M2 ? d + 16 : 2 * d + 16) + 2 * d * w.keys) * 2;
@@ -1413,15 +1419,15 @@ template <int D, int MODE, bool PAGE16, bool ZS>
 __global__ __launch_bounds__(256, wide_shape(D).occ) void chunk_mixed_kernel(ChunkArgs a, int n_slots) {
     constexpr int NB = mixed_blocks(D);
     int bid = blockIdx.x;
-    const int wide = n_slots * a.n_kv_heads * (ZS ? a.z_wide : 1), pairs = a.n_seq * a.n_kv_heads, narrow = pairs * a.z_narrow;
+    const int wide = n_slots * a.n_kv_heads * (ZS ? a.z_wide : 1), pairs = a.n_seq * a.n_kv_heads, ranges = pairs * a.z_narrow, narrow = ranges * a.narrow_tiles;
     if (bid < wide) {
         chunk_wide_body<D, MODE, PAGE16, ZS>(a, bid);
         return;
     }
     bid -= wide;
     if (bid < narrow) {
-        const int zr = bid / pairs;
-        chunk_narrow_body<D, MODE, NB, PAGE16 ? ring_steps(D, NB) : 0>(a, bid - zr * pairs, 0, zr);
+        const int tile = bid / ranges, at = bid - tile * ranges, zr = at / pairs;
+        chunk_narrow_body<D, MODE, NB, PAGE16 ? ring_steps(D, NB) : 0>(a, at - zr * pairs, tile, zr);
     } else {
         chunk_fill_outside<D>(a, bid - narrow, gridDim.x - wide - narrow, 256);
     }
@@ -1594,12 +1600,12 @@ static ChunkPlan chunk_plan(int64_t n_seq, int64_t total_rows, int64_t n_q_heads
     } else {
         p.wide = true;
         p.nb = mixed_blocks((int)d);
-        p.tiles = 1;
+        p.tiles = mixed_tiles((int)d);
         // with n_seq - 1 sequences of the longest length, can the last one be short?  (If the hint is wrong the LDS kernel
         // takes the short ones too.)
         const int64_t least = total_rows - (n_seq - 1) * rows_most;
-        p.narrow = n_seq > 1 && (least < 1 ? 1 : least) * group <= 16 * p.nb;   // (one row has `group` columns)
-        p.col_split = p.narrow ? 16 * p.nb : 0;
+        p.narrow = n_seq > 1 && (least < 1 ? 1 : least) * group <= 16 * p.nb * p.tiles;   // (one row has `group` columns)
+        p.col_split = p.narrow ? 16 * p.nb * p.tiles : 0;
     }
     p.narrow_rows = p.wide && p.narrow ? (int)(p.col_split / group) : 0;
     const int64_t each = n_seq > 0 ? (total_rows + n_seq - 1) / n_seq * group : 1;   // columns of a sequence of average length
@@ -1646,7 +1652,7 @@ static int launch_chunk_wide(const ChunkArgs &a, bool narrow, bool fill, hipStre
     constexpr int NB = mixed_blocks(D), RING = PAGE16 ? ring_steps(D, NB) : 0;
     constexpr bool kOneGrid = w.waves == 4;            // both kernels' workgroups have four waves
     const int64_t slots = chunk_slots(a.total_rows, a.n_seq, a.group, w.columns);
-    const int64_t wide = slots * a.n_kv_heads * a.z_wide, more = narrow && kOneGrid ? (int64_t)a.n_seq * a.n_kv_heads * a.z_narrow : 0;
+    const int64_t wide = slots * a.n_kv_heads * a.z_wide, more = narrow && kOneGrid ? (int64_t)a.n_seq * a.n_kv_heads * a.narrow_tiles * a.z_narrow : 0;
     FEATHER_CHECK(wide + more + kChunkFillGroups < (1ll << 31), FEATHER_ESHAPE, "feather_paged_chunk_attn_fp8: grid too large");
     const dim3 grid((unsigned)(wide + more + (fill ? kChunkFillGroups : 0)));
     if constexpr (kOneGrid)

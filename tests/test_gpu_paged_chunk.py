@@ -130,6 +130,9 @@ SHAPES = [
     ([25], [900], 4, 1, 128, 16),
     ([15], [600], 4, 1, 256, 16),
     ([9], [700], 3, 1, 512, 16),
+    ([5, 8, 70, 1], [300, 1500, 900, 40], 8, 1, 64, 16),  # drafts of more than one tile beside a chunk
+    ([8, 70, 7], [1100, 70, 9], 8, 1, 64, 20),
+    ([10, 16, 60], [700, 90, 1300], 4, 1, 128, 16),
     ([4], [2049], 16, 1, 64, 16),                         # few columns, a long cache: ranges
     ([1, 1, 1], [3000, 1, 777], 8, 1, 128, 16),
 ]
