@@ -1490,6 +1490,9 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(ChunkArgs a, int qt_wi
         }
     }
     const float2p_t *ml = reinterpret_cast<const float2p_t *>(part + z * part_items * D);
+    // A range without a maximum has only hidden keys (sum and accumulators are zero) or only NaN scores (then they are NaN,
+    // and so is the row): its weight is zero, which keeps a NaN, and it is not left out.
+    auto weight = [&](float m_range, float m_all) { return m_range == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_range - m_all) * a.scale_log2e); };
     float m = -INFINITY, l = 0.f;
     float4_t acc = {0.f, 0.f, 0.f, 0.f};
     for (int z0 = zi; z0 < used; z0 += G * zl) {       // G ranges per turn, all loads before the first use
@@ -1507,13 +1510,13 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(ChunkArgs a, int qt_wi
             if (z0 + g * zl >= used) x[g] = float2p_t{-INFINITY, 0.f};
             mg = fmaxf(mg, x[g][0]);
         }
-        const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mg) * a.scale_log2e);
+        const float keep = weight(m, mg);
         l *= keep;
         acc *= keep;
 #pragma unroll
         for (int g = 0; g < G; g++) {
-            if (x[g][0] == -INFINITY) continue;        // a range of hidden keys only
-            const float w = __builtin_amdgcn_exp2f((x[g][0] - mg) * a.scale_log2e);
+            if (z0 + g * zl >= used) continue;
+            const float w = weight(x[g][0], mg);
             l += x[g][1] * w;
             acc += y[g] * w;
         }
@@ -1526,13 +1529,12 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(ChunkArgs a, int qt_wi
         if (zi > 0) return;
         float mg = m;
         for (int k = 1; k < zl; k++) mg = fmaxf(mg, ml_lds[tid + k * DW][0]);
-        const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mg) * a.scale_log2e);
+        const float keep = weight(m, mg);
         l *= keep;
         acc *= keep;
         for (int k = 1; k < zl; k++) {
             const float2p_t x = ml_lds[tid + k * DW];
-            if (x[0] == -INFINITY) continue;
-            const float w = __builtin_amdgcn_exp2f((x[0] - mg) * a.scale_log2e);
+            const float w = weight(x[0], mg);
             l += x[1] * w;
             acc += x_lds[tid + k * DW] * w;
         }
