@@ -14,8 +14,10 @@
 //
 // Numerics.  fp16 x fp16 (or bf8 x bf8) products summed in fp32, softmax statistics in fp32.  P is rounded to fp16
 // (nearest even) before it multiplies V, as in the other attention kernels: the second product then runs at the fp16
-// rate, and the error (2^-11 / sqrt(3) of each P, random in sign) is of the size of the fp16 result's own rounding.
-// The denominator sums the rounded P.
+// rate, and the error (at most 2^-11 of each P) is of the size of the fp16 result's own rounding.  The denominator sums
+// the rounded P.  P is scaled so that the largest one is 2^8 or more (kShift): then a P of 2^-22 of the largest is still a
+// normal half, one below it is off by at most 2^-33 of the largest, and none above 2^-33 vanishes.  (With the largest at
+// 1, many equal keys at 2^-25 of one dominating key were lost altogether.)
 //
 // Kernels.  Many columns: K and V tiles through LDS, shared by a workgroup's waves -- chunk_attn32_body (d = 64, 128) on
 // the 32x32 matrix instructions, chunk_attn_body (d = 256, 512) on the 16x16 ones.  Few columns: chunk_narrow_body, where
@@ -190,9 +192,13 @@ __device__ __forceinline__ int narrow_min_keys(const ChunkArgs &a, int qt) {
     return max((per / kNarrowStep + 1) * kNarrowStep, kNarrowMinKeys);
 }
 
-// A column's P = 2^((s - m) c) refers to a point m that need not be its maximum: O / l does not depend on it.  A lane's P
-// are positive, so a sum below kGuard bounds each of them, far from fp16's largest value.
-constexpr float kGuard = 4096.f;
+// A column's P = 2^((s - m) c + kShift) refers to a point m that need not be its maximum: O / l does not depend on it, nor
+// on kShift, which is the same in every wave and range.  A lane's P are positive, so a sum below kGuard bounds each of them
+// by fp16's largest value, 65504; 32 P of 2^kShift sum to 2^13, so a column's scores can grow by a factor of 2^2.9 (all
+// equal) to 2^7.9 (one large) before the reference is raised.
+constexpr float kShift = 8.f, kGuard = 61440.f;
+constexpr float kLazy = 7.f;           // the kernel that compares maxima raises the reference beyond 2^kLazy: P to 2^(kShift + kLazy) = 32768
+__device__ __forceinline__ float chunk_reference(float m, float scale_log2e) { return __builtin_fmaf(m, scale_log2e, -kShift); }
 constexpr int kAnyColumns = 1 << 30;   // more columns than a call can have
 
 // ---- tiles through LDS --------------------------------------------------------------------------------------------
@@ -278,7 +284,7 @@ __device__ __forceinline__ void chunk_attn_body(const ChunkArgs &a, int bid) {
 #pragma unroll
         for (int d = 0; d < DB; d++) o[b][d] = float4_t{0.f, 0.f, 0.f, 0.f};
     }
-    const float lazy_raw = 8.f / a.scale_log2e;
+    const float lazy_raw = kLazy / a.scale_log2e;
 
     u32x4 kreg[NU];
     uint32_t vreg[NU][4];
@@ -437,12 +443,12 @@ __device__ __forceinline__ void chunk_attn_body(const ChunkArgs &a, int bid) {
                     mx = max3_raw(mx, s[b][c][2], s[b][c][3]);
                 }
                 mx = max_xor32(max_xor16(mx));
-                // The reference point is raised only when a column exceeds it by 2^8 (O / l does not depend on it).  A
+                // The reference point is raised only when a column exceeds it by 2^kLazy (O / l does not depend on it).  A
                 // column that has seen no key yet keeps -inf and refers to zero: its scores are -inf, its P zero.
                 const float m_old = m_run[b];
                 const bool raise = __builtin_amdgcn_ballot_w64(mx > m_old + lazy_raw) != 0;
                 const float m_new = raise ? max_raw(m_old, mx) : m_old;
-                const float mc = m_new == -INFINITY ? 0.f : m_new * a.scale_log2e;
+                const float mc = m_new == -INFINITY ? 0.f : chunk_reference(m_new, a.scale_log2e);
                 if (raise) {
                     const float alpha = m_old == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_old - m_new) * a.scale_log2e);
                     m_run[b] = m_new;
@@ -611,7 +617,7 @@ __device__ __forceinline__ void chunk_attn32_body(const ChunkArgs &a, int bid) {
     }
 
     float16_t o[CB][DB];                         // [32-dim block]
-    float m_run[CB], mc_run[CB], l_run[CB];      // reference point (raw, and times scale * log2 e), the lane's share of the sum
+    float m_run[CB], mc_run[CB], l_run[CB];      // reference point (raw, and as chunk_reference gives it), the lane's share of the sum
 #pragma unroll
     for (int b = 0; b < CB; b++) {
         m_run[b] = mc_run[b] = -INFINITY;
@@ -819,7 +825,7 @@ __device__ __forceinline__ void chunk_attn32_body(const ChunkArgs &a, int bid) {
                     // a column that has seen no key keeps the reference -inf: its scores are -inf here, its P zero
                     const float alpha = m_old == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_old - m_new) * a.scale_log2e);
                     m_run[b] = m_new;
-                    mc_run[b] = m_new * a.scale_log2e;
+                    mc_run[b] = chunk_reference(m_new, a.scale_log2e);
                     l_run[b] *= alpha;
 #pragma unroll
                     for (int d = 0; d < DB; d++) o[b][d] *= alpha;
@@ -1119,7 +1125,7 @@ __device__ __forceinline__ void chunk_narrow_body(const ChunkArgs &a, int pair, 
     const int tile_first = a.causal ? t.p0 + chunk_row_of(a, t.col0) : t.ctx - 1;
 
     float4_t o[NB][RB][4];
-    float m_run[NB], mc_run[NB], l_run[NB];   // reference point (raw, and times scale * log2 e), the lane's share of the sum
+    float m_run[NB], mc_run[NB], l_run[NB];   // reference point (raw, and as chunk_reference gives it), the lane's share of the sum
 #pragma unroll
     for (int b = 0; b < NB; b++) {
         m_run[b] = mc_run[b] = -INFINITY;
@@ -1215,7 +1221,7 @@ __device__ __forceinline__ void chunk_narrow_body(const ChunkArgs &a, int pair, 
                 // a column that has seen no key keeps the reference -inf: its scores are -inf here, its P zero
                 const float alpha = m_old == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_old - m_new) * a.scale_log2e);
                 m_run[b] = m_new;
-                mc_run[b] = m_new * a.scale_log2e;
+                mc_run[b] = chunk_reference(m_new, a.scale_log2e);
                 l_run[b] *= alpha;
 #pragma unroll
                 for (int rb = 0; rb < RB; rb++)

@@ -12,7 +12,7 @@ pytestmark = pytest.mark.gpu
 NAN = 0x7F
 
 
-def _run(P, dev, size, kind, causal=1):
+def _run(P, dev, size, kind, scale=None):
     """Through the C ABI with a workspace of `size` bytes (None: as many as the call asks for); fp32 or fp16 results."""
     from feather_amd import _native as N
     t = [torch.from_numpy(np.ascontiguousarray(P[k]).view(np.int32).copy()).to(dev) for k in ("q", "kc", "vc", "bt", "cu", "ctx")]
@@ -23,7 +23,8 @@ def _run(P, dev, size, kind, causal=1):
     ws = torch.empty(max(size, 16), dtype=torch.uint8, device=dev)
     out = torch.full((P["total"], P["Hq"], P["d"]), 7.0, device=dev, dtype=torch.float32 if kind == N.CHUNK_OUT_F32 else torch.float16)
     N.check(L.feather_paged_chunk_attn_fp8(*[x.data_ptr() for x in t], out.data_ptr(), kind, 0, ws.data_ptr() if size else None, size,
-                                           *shape, P["bs"], mb, P["kc"].shape[0], 0, causal, N.E5M2, P["d"] ** -0.5, N.stream_ptr(dev)))
+                                           *shape, P["bs"], mb, P["kc"].shape[0], 0, 1, N.E5M2, P["d"] ** -0.5 if scale is None else float(scale),
+                                           N.stream_ptr(dev)))
     torch.cuda.synchronize()
     return out.double().cpu(), need
 
