@@ -3,7 +3,8 @@
 // layers), with no host copy of the tables and no atomics whose order shows:
 //   fork     slot i of a batch goes on as a copy of slot parents[i] (beam search, samples of one prompt, reordering;
 //            -1 ends the slot).  Whole blocks are shared; the block that a context ends in is copied for every child but
-//            the first, because each child will write its own next token there.  Then room is reserved.
+//            the first, because each child will write its own next token there -- and for the first too if another entry
+//            or a pin holds that block, as after a length was set back into shared blocks.  Then room is reserved.
 //   compact  the blocks in use move to the lowest ids, so that the upper part of the pool is free.
 // Both return new tables, counts and maps and change none of those they are given; only cache blocks that were free
 // are written.  Free blocks are handed out lowest id first in (slot, entry) order, so results are those of a serial loop.
@@ -25,7 +26,7 @@ namespace feather {
 constexpr int kPgThreads = 256;
 constexpr int kPgMaxCaches = 64;          // caches of one launch (their pointers travel with the kernel's arguments)
 constexpr int kPgChunkThreads = 1024;
-constexpr int kPgMinChunk = 1024, kPgMaxChunks = 256, kPgMaxChunk = 16384;
+constexpr int kPgMinChunk = kPgChunkThreads, kPgMaxChunks = 256, kPgMaxChunk = 16384;
 constexpr int kPgMaxSlots = 8192;
 
 struct CachePtrs {
@@ -80,24 +81,39 @@ struct ForkArgs {
 constexpr int kFreshTail = -2, kFreshRoom = -3;   // entries of a new row that still wait for a block
 
 // Workgroups [0, chunks): reference counts and free blocks of a chunk of the pool.  An old row p with n children
-// passes its whole blocks on to all of them, the rest of its entries to the first: an entry's count changes by
-// n - 1, or by (n > 0) - 1.  Workgroups from `chunks` on: the new row of one slot, with marks for fresh blocks.
+// passes its whole blocks on to all of them, the rest of its entries to the first, but no block of the rest that is
+// held by others as well (its count was above 1, a bit of `held`): an entry's count changes by n - 1, or by 0 if passed on
+// and -1 if not.  Such a block under the end of a context is copied for the first child too (a bit of `source`): should its
+// count come to 0, it is free only after this call.  Counts as they were decide, not those that remain when other rows have
+// let go: those would be known only when all chunks are done, a third launch; the price is a copy that could be spared when
+// the other holders end in the same call.  Workgroups from `chunks` on: the new row of one slot, with marks for fresh
+// blocks.
 __global__ __launch_bounds__(kPgChunkThreads) void fork_plan_kernel(ForkArgs a) {
     extern __shared__ __attribute__((aligned(16))) int pg_lds[];
     __shared__ int red[kPgChunkThreads / kWave];
     const int tid = threadIdx.x, cap = a.max_blocks * a.block_size;
     if ((int)blockIdx.x < a.chunks) {
-        int *count = pg_lds, *children = pg_lds + a.chunk, *whole = children + a.n_seq;
+        int *count = pg_lds;
+        int2 *row = reinterpret_cast<int2 *>(pg_lds + a.chunk);        // children; 2 * whole blocks + (1: a part of one more)
+        uint32_t *held = reinterpret_cast<uint32_t *>(row + a.n_seq), *source = held + a.chunk / 32;
         const int b0 = blockIdx.x * a.chunk, n = min(a.chunk, a.n_blocks - b0);
-        for (int i = tid; i < n; i += kPgChunkThreads) count[i] = a.ref[b0 + i];
+        for (int i = tid; i < a.chunk; i += kPgChunkThreads) {          // (a chunk is a multiple of the workgroup)
+            const int r = i < n ? a.ref[b0 + i] : 0;
+            const uint64_t m = __builtin_amdgcn_ballot_w64(r > 1);
+            count[i] = r;
+            if (lane_id() < 2) {
+                held[i / 64 * 2 + lane_id()] = (uint32_t)(m >> (32 * lane_id()));
+                source[i / 64 * 2 + lane_id()] = 0;
+            }
+        }
         for (int i = tid; i < a.n_seq; i += kPgChunkThreads) {
-            children[i] = 0;
-            whole[i] = min(max(a.ctx_lens[i], 0), cap) / a.block_size;
+            const int len = min(max(a.ctx_lens[i], 0), cap);
+            row[i] = int2{0, 2 * (len / a.block_size) + (len % a.block_size != 0)};
         }
         __syncthreads();
         for (int i = tid; i < a.n_seq; i += kPgChunkThreads) {
             const int p = a.parents[i];
-            if ((unsigned)p < (unsigned)a.n_seq) atomicAdd(&children[p], 1);
+            if ((unsigned)p < (unsigned)a.n_seq) atomicAdd(&row[p].x, 1);
         }
         __syncthreads();
         constexpr int G = 8;                           // table entries in flight per thread
@@ -110,49 +126,66 @@ __global__ __launch_bounds__(kPgChunkThreads) void fork_plan_kernel(ForkArgs a) 
             for (int g = 0; g < G; g++) {
                 const int i = i0 + g * kPgChunkThreads;
                 if (i >= entries || (unsigned)v[g] >= (unsigned)n) continue;
-                const int p = (int)(__umulhi(2u * (uint32_t)i, a.row_mul) >> a.row_shift), e = i - p * a.max_blocks, kids = children[p];
-                const int change = (e < whole[p] ? kids : (kids > 0 ? 1 : 0)) - 1;
+                const int p = (int)(__umulhi(2u * (uint32_t)i, a.row_mul) >> a.row_shift), e = i - p * a.max_blocks;
+                const int2 r = row[p];                 // (one read of 64 bits: the LDS bounds this loop)
+                int change = r.x - 1;
+                if (2 * e + 1 >= r.y) {                // not a whole block of the context
+                    change = -1;
+                    if (r.x > 0) {
+                        const uint32_t bit = 1u << (v[g] & 31);
+                        if (!(held[v[g] >> 5] & bit)) change = 0;
+                        else if (2 * e + 1 == r.y) atomicOr(&source[v[g] >> 5], bit);
+                    }
+                }
                 if (change) atomicAdd(&count[v[g]], change);
             }
         }
         __syncthreads();
         const int per = (n + kPgChunkThreads - 1) / kPgChunkThreads, i0 = min(tid * per, n), i1 = min(i0 + per, n);
+        auto is_free = [&](int i) { return count[i] == 0 && !(source[i >> 5] >> (i & 31) & 1); };
         int mine = 0;
         for (int i = i0; i < i1; i++) {
             a.ref_out[b0 + i] = count[i];
-            mine += count[i] == 0;
+            mine += is_free(i);
         }
         int total;
         int at = pg_block_scan(mine, red, kPgChunkThreads, &total);
         for (int i = i0; i < i1; i++)
-            if (count[i] == 0) a.free_ids[b0 + at++] = b0 + i;
+            if (is_free(i)) a.free_ids[b0 + at++] = b0 + i;
         if (tid == 0) a.free_count[blockIdx.x] = total;
         return;
     }
     const int i = blockIdx.x - a.chunks, p = a.parents[i];
     const bool alive = (unsigned)p < (unsigned)a.n_seq;
-    int earlier = 0;
+    auto entry_of = [&](int e, int &v, int &count) {   // the parent's entry, -1 for what is no block, and the block's count
+        v = alive && e < a.max_blocks ? a.tables[(int64_t)p * a.max_blocks + e] : -1;
+        if ((unsigned)v >= (unsigned)a.n_blocks) v = -1;
+        count = v >= 0 ? a.ref[v] : 0;
+    };
+    int v_next, count_next, earlier = 0;
+    entry_of(tid, v_next, count_next);                 // requested before the vote, which waits for all earlier parents
     if (alive)
         for (int k = tid; k < i; k += kPgChunkThreads) earlier |= a.parents[k] == p;
-    const bool heir = !__syncthreads_or(earlier) && alive;
     const int len = alive ? min(max(a.ctx_lens[p], 0), cap) : 0;
+    const bool heir = !__syncthreads_or(earlier) && alive;
     const int whole = len / a.block_size, used = (len + a.block_size - 1) / a.block_size;
     const int wanted = a.room ? max(a.room[i], 0) : 0;
     const int want = wanted >= cap ? a.max_blocks : (wanted + a.block_size - 1) / a.block_size;
     int fresh = 0, hole = 0, tail = 0;
     for (int e = tid; e < a.max_blocks; e += kPgChunkThreads) {
-        int v = -1;
-        if (alive && (e < whole || heir || (e == whole && used > whole))) v = a.tables[(int64_t)p * a.max_blocks + e];
-        if ((unsigned)v >= (unsigned)a.n_blocks) v = -1;
+        int v = v_next;
+        const bool own = heir && (e < whole || count_next <= 1);   // may stay in the slot's row as it is
+        entry_of(e + kPgChunkThreads, v_next, count_next);
         if (e < used) {
             hole |= v < 0;
-            if (!heir && e == whole && v >= 0) {
+            if (!own && e == whole && v >= 0) {
                 a.source[i] = v;
                 v = kFreshTail;
                 tail = 1;
             }
-        } else if (v < 0 && e < want) {
-            v = kFreshRoom;
+        } else {
+            if (!own) v = -1;
+            if (v < 0 && e < want) v = kFreshRoom;
         }
         fresh += v < -1;
         a.tables_out[(int64_t)i * a.max_blocks + e] = v;
@@ -387,12 +420,12 @@ extern "C" int feather_paged_cache_fork(const void *const *caches_host, int64_t 
     a.need = (int32_t *)scratch; a.source = a.need + n_seq; a.free_count = a.source + n_seq; a.free_ids = a.free_count + kPgMaxChunks;
     a.n_seq = (int)n_seq; a.max_blocks = (int)max_blocks; a.block_size = (int)block_size; a.n_blocks = (int)n_blocks;
     a.chunk = (int)pg_chunk(n_blocks); a.chunks = (int)((n_blocks + a.chunk - 1) / a.chunk);
-    const size_t lds = ((size_t)a.chunk + 2 * n_seq) * 4;
+    const size_t lds = ((size_t)a.chunk + 2 * n_seq + a.chunk / 16) * 4;   // counts, two words per slot, two bits per block
     a.row_shift = 0;
     while ((1ll << a.row_shift) < max_blocks) a.row_shift++;
     a.row_mul = max_blocks > 0 ? (uint32_t)((1ull << (31 + a.row_shift)) / (uint64_t)max_blocks + 1) : 0;
     static unsigned long long lds_raised = 0;
-    hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(fork_plan_kernel), (size_t)(kPgMaxChunk + 2 * kPgMaxSlots) * 4, lds_raised);
+    hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(fork_plan_kernel), (size_t)(kPgMaxChunk + 2 * kPgMaxSlots + kPgMaxChunk / 16) * 4, lds_raised);
     FEATHER_CHECK(e == hipSuccess, FEATHER_ELAUNCH, "%s: cannot raise LDS limit: %s", me, hipGetErrorString(e));
     hipStream_t s = (hipStream_t)stream;
     hipLaunchKernelGGL(fork_plan_kernel, dim3((unsigned)(a.chunks + n_seq)), dim3(kPgChunkThreads), lds, s, a);

@@ -168,7 +168,8 @@ class PackedDecoder:
 
         token_ids     ``[total_rows]`` int32; sequence ``s`` brings ``token_ids[cu[s] : cu[s+1]]``
         block_tables  ``[n_seq, max_blocks]`` int32; must have blocks for the new tokens, and no two sequences may share
-                      a block that one of them writes (:meth:`fork` with ``room`` sees to both)
+                      a block that one of them writes (:meth:`fork` with ``room`` sees to both; also after lengths were
+                      set back below those at the last fork)
         ctx_lens      ``[n_seq]`` int32 tokens already cached; the new ones get the positions behind them
         rows          int32 rows whose logits are wanted (default: the last row of each sequence)
         max_q_len     a bound of a sequence's rows, if known; it only helps to choose the kernels

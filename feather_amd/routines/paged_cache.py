@@ -70,7 +70,9 @@ def paged_cache_fork(caches, block_tables: torch.Tensor, ctx_lens: torch.Tensor,
     room        optional ``[n_seq]`` int32: positions the slot's row must cover afterwards (fresh blocks are added)
     Returns ``(block_tables, ctx_lens, ref_counts, status)``.  Whole blocks of a context are shared by all children; the
     block it ends in stays with the first child of a parent and is copied for the others, because each of them writes its
-    next token there.  Fresh blocks are taken lowest id first in (slot, entry) order.  ``status``: 0; 1 ``room`` beyond
+    next token there; the first child gets a copy too if another entry or a pin holds that block (``ref_counts`` above 1),
+    and entries behind the context that are held so are dropped.  That happens when a length was set back into blocks that
+    an earlier fork shared: such a slot must go through this call (as its own parent) before the next append.  Fresh blocks are taken lowest id first in (slot, entry) order.  ``status``: 0; 1 ``room`` beyond
     the table; 2 a table entry within the context is not a block; 3 the pool ran out (the missing entries are -1, and a
     slot that lost the copy of its last block keeps its whole blocks as its length).  ``ref_counts`` must count the rows
     of ``block_tables``."""

@@ -383,7 +383,10 @@ int feather_rope_append_chunk(const void *qkv, int src_f16, int64_t row_stride, 
  *
  * feather_paged_cache_fork: slot i becomes a copy of slot parents[i] of the old state ([n_seq] int32; a value outside
  * [0, n_seq) ends the slot: an empty row, length 0).  Blocks that a context fills are shared by all children.  The first child (lowest i) of a
- * parent takes the rest of its row too; every other child gets a copy of the block its context ends in.  Then, if room
+ * parent takes the rest of its row too; every other child gets a copy of the block its context ends in.  So does the first
+ * one if ref_counts is above 1 for that block (another entry or a pin holds it, as after ctx_lens was set back into blocks
+ * that a fork shared), and entries past the context whose blocks are held so are dropped: where a slot writes next, no other
+ * does.  A block copied from for that reason is not handed out in the same call.  Then, if room
  * ([n_seq] int32) is given, entries past the context are filled with fresh blocks until the row covers room[i] positions.
  * Fresh blocks are the free ones (after the old rows have let go), lowest id first, in (slot, entry) order.  Entries that
  * are not blocks come out as -1.  seq_status (or NULL): 0; 1 = room[i] beyond the table (filled to its end); 2 = an entry
