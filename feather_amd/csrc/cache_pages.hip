@@ -6,8 +6,10 @@
 //            the first, because each child will write its own next token there -- and for the first too if another entry
 //            or a pin holds that block, as after a length was set back into shared blocks.  Then room is reserved.
 //   compact  the blocks in use move to the lowest ids, so that the upper part of the pool is free.
-// Both return new tables, counts and maps and change none of those they are given; only cache blocks that were free
-// are written.  Free blocks are handed out lowest id first in (slot, entry) order, so results are those of a serial loop.
+// Both return new tables, counts and maps and change none of those they are given.  Of the caches only blocks that no new
+// row holds are written: those free before, and in a fork also those that this very call releases, so the old tables are
+// void after it, also when the pool ran out.  Free blocks are handed out lowest id first in (slot, entry) order, so results
+// are those of a serial loop.
 //
 // Integer part: every chunk of the pool is one workgroup that reads all tables once and counts in LDS, beside one
 // workgroup per slot that lays out the slot's new row.  The tables and counts are read from the L2, so a read is a round

@@ -4,7 +4,8 @@ reference has no KV cache.
 
 The state is a block table ``[n_seq, max_blocks]`` int32 (-1: no block), the lengths ``ctx_lens [n_seq]`` int32 and
 ``ref_counts [n_blocks]`` int32: how many table entries (and pins of the caller) hold a block, 0 = free.  Calls return new
-tables, lengths and counts; the caches are updated in place, in blocks that were free.  Nothing is copied to the host.
+tables, lengths and counts; the caches are updated in place, in blocks that were free or that the call releases: after a
+fork the tables passed in are void.  Nothing is copied to the host.
 """
 from __future__ import annotations
 
@@ -72,10 +73,12 @@ def paged_cache_fork(caches, block_tables: torch.Tensor, ctx_lens: torch.Tensor,
     block it ends in stays with the first child of a parent and is copied for the others, because each of them writes its
     next token there; the first child gets a copy too if another entry or a pin holds that block (``ref_counts`` above 1),
     and entries behind the context that are held so are dropped.  That happens when a length was set back into blocks that
-    an earlier fork shared: such a slot must go through this call (as its own parent) before the next append.  Fresh blocks are taken lowest id first in (slot, entry) order.  ``status``: 0; 1 ``room`` beyond
-    the table; 2 a table entry within the context is not a block; 3 the pool ran out (the missing entries are -1, and a
-    slot that lost the copy of its last block keeps its whole blocks as its length).  ``ref_counts`` must count the rows
-    of ``block_tables``."""
+    an earlier fork shared: such a slot must go through this call (as its own parent) before the next append.  Fresh blocks
+    are taken lowest id first in (slot, entry) order.  ``status``: 0; 1 ``room`` beyond the table; 2 a table entry within
+    the context is not a block; 3 the pool ran out (the missing entries are -1, and a slot that lost the copy of its last
+    block keeps its whole blocks as its length).  ``ref_counts`` must count the rows of ``block_tables``.  Blocks that the
+    old rows let go may be handed out and written in the same call, so the tables passed in are void after it, also with
+    status 3: a slot that must survive needs a child."""
     ref_counts = _index(ref_counts, "ref_counts")
     ptrs, n_caches, block_bytes, block_size = _pool(caches, ref_counts)
     block_tables = _index(block_tables, "block_tables")

@@ -379,7 +379,7 @@ int feather_rope_append_chunk(const void *qkv, int src_f16, int64_t row_stride, 
  * ref_counts [n_blocks] int32: how many table entries (and pins of the caller) hold a block; 0 = free.  caches_host is a
  * HOST array of n_caches device pointers, every cache [n_blocks] blocks of block_bytes bytes (a multiple of 16): K and V
  * of all layers that share the tables.  Tables, counts and lengths are read from their inputs and written to separate
- * outputs; of the caches only blocks that were free are written.  n_blocks <= 4194304.
+ * outputs; of the caches only blocks that were free are written, or that the same call releases.  n_blocks <= 4194304.
  *
  * feather_paged_cache_fork: slot i becomes a copy of slot parents[i] of the old state ([n_seq] int32; a value outside
  * [0, n_seq) ends the slot: an empty row, length 0).  Blocks that a context fills are shared by all children.  The first child (lowest i) of a
@@ -391,7 +391,10 @@ int feather_rope_append_chunk(const void *qkv, int src_f16, int64_t row_stride, 
  * Fresh blocks are the free ones (after the old rows have let go), lowest id first, in (slot, entry) order.  Entries that
  * are not blocks come out as -1.  seq_status (or NULL): 0; 1 = room[i] beyond the table (filled to its end); 2 = an entry
  * within the context is not a block; 3 = the pool ran out (missing entries are -1; a slot that lost the copy of its last
- * block keeps its whole blocks as its length).  ref_counts must count the rows of block_tables.  n_seq <= 8192. */
+ * block keeps its whole blocks as its length).  ref_counts must count the rows of block_tables.  n_seq <= 8192.
+ * Blocks that the old rows let go (of ended slots, or replaced by copies) may hold other data after the call, whatever
+ * seq_status says: the tables that were passed in are void, and a caller who wants to retry after a 3 goes on from the new
+ * ones.  A slot that must survive a fork that may run out needs a child in it. */
 int64_t feather_paged_cache_fork_scratch_bytes(int64_t n_seq, int64_t n_blocks);
 int feather_paged_cache_fork(const void *const *caches_host, int64_t n_caches, int64_t block_bytes, const void *block_tables,
                              const void *ctx_lens, const void *ref_counts, const void *parents, const void *room,

@@ -129,6 +129,25 @@ def test_two_slots_set_back_into_one_block(dev):
         assert np.array_equal(a, b)
 
 
+def test_what_a_fork_that_runs_out_leaves_of_the_old_state(dev):
+    """Blocks of ended slots are handed out in the same call and may be written; what a new row holds is as it was."""
+    rng = np.random.default_rng(3)
+    bt = np.array([[0, 1, -1], [2, 3, -1], [4, 5, 6]], np.int32)
+    ctx = np.array([6, 7, 12], np.int32)
+    ref = np.ones(7, np.int32)                                 # blocks of 4 tokens, nothing free
+    caches = [rng.integers(0, 2 ** 32, (7, 1, 4, 4), dtype=np.uint64).astype(np.uint32) for _ in range(2)]
+    parents, room = np.array([0, 0, 2], np.int32), np.array([9, 9, 12], np.int32)
+    want = fork_loop(caches, bt, ctx, ref, parents, room, 4)
+    got, after = _fork(dev, bt, ctx, ref, caches, parents, room)
+    _same(got, after, want)
+    tables, lens, counts, status = got
+    # slot 1's blocks 2 and 3 go to the spare entry of slot 0 and to the copy of block 1; then the pool is empty
+    assert tables.tolist() == [[0, 1, 2], [0, 3, -1], [4, 5, 6]] and status.tolist() == [0, 3, 0] and lens.tolist() == [6, 6, 12]
+    for a, c in zip(after, caches):
+        assert np.array_equal(a[3], c[1]) and not np.array_equal(a[3], c[3])   # an old row of an ended slot is void
+        assert all(np.array_equal(a[b], c[b]) for b in (0, 1, 2, 4, 5, 6))      # (block 2 is reserved, not written)
+
+
 @pytest.mark.parametrize("mode,head_dim,block", [("E4M3", 64, 16), ("E5M2", 128, 16)])
 def test_drafts_rejected_across_a_fork(mode, head_dim, block):
     """Two samples of a prompt whose tail was itself a draft: both go back behind the fork, fork again, and go on alone."""
