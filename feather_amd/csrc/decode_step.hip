@@ -17,6 +17,7 @@
 // touches memory.  All launches go to one stream; nothing allocates or syncs.
 #include "internal.h"
 #include "common.h"
+#include "rotary.h"
 
 namespace feather {
 
@@ -193,23 +194,8 @@ __global__ __launch_bounds__(kDsThreads) void swiglu_pack_kernel(const float *__
 // status[b] says why (1: no room / bad position, 2: bad block id; 0: appended).  pos_limit is the number of
 // positions the caller's context bound allows (at most the table's max_blocks * block_size).
 constexpr int kRopeThreads = 64;
-// sin and cos of a non-negative angle below ~1e5 rad to ~1e-7 absolute: three-constant Cody-Waite reduction
-// by pi/2 with fused multiply-adds, then the single-precision minimax polynomials on [-pi/4, pi/4].  The
-// library's sincosf (full range reduction) was the longest phase of the RoPE kernel: 1.3 of its 2.2 us.
-__device__ __forceinline__ void sincos_small(float x, float &s, float &c) {
-    const float k = rintf(x * 0.636619772f);
-    float r = fmaf(k, -1.57079625e+00f, x);
-    r = fmaf(k, -7.54978942e-08f, r);
-    r = fmaf(k, -5.39030295e-15f, r);
-    const float r2 = r * r;
-    const float sp = fmaf(r * r2, fmaf(r2, fmaf(r2, -1.9515295891e-4f, 8.3321608736e-3f), -1.6666654611e-1f), r);
-    const float cp = fmaf(r2, fmaf(r2, fmaf(r2, fmaf(r2, 2.443315711809948e-5f, -1.388731625493765e-3f), 4.166664568298827e-2f), -0.5f), 1.0f);
-    const int q = (int)k;
-    const float ss = (q & 1) ? cp : sp, cc = (q & 1) ? sp : cp;
-    s = (q & 2) ? -ss : ss;
-    c = ((q + 1) & 2) ? -cc : cc;
-}
-
+// (Sine and cosine: sincos_small.  The library's sincosf, with its full range reduction, was the longest phase of the
+// RoPE kernel: 1.3 of its 2.2 us.)
 // (parameter order: everything needed before the first loads sits in the 16 preloaded dwords)
 template <int MODE>
 __global__ __launch_bounds__(kRopeThreads) void rope_append_kernel(const float *__restrict__ qkv,

@@ -4,7 +4,8 @@
 //     (a, b) -> amplitude * (a cos t - b sin t, b cos t + a sin t),   t = 2 pi * position * freq[pair]
 // Pairs are (j, j + rot_dim / 2) (half layout) or (2j, 2j + 1) (interleaved).  freq is in turns per position and in
 // 64 bits, and so is the product: far positions make thousands of turns, of which only the fraction counts (a 32-bit
-// product at position 10^5 is off by 2^-8 of a turn).  The fraction is exact to 2^-53 * turns; from there on 32 bits do.
+// product around position 10^5 is off by up to 0.001 of a turn).  The fraction is exact to 2^-53 * turns; from there on
+// 32 bits do.
 //
 // A streaming kernel, bound by its bytes: 4 (or 2) in, 1 out per element.  The angles of a token are computed once per
 // workgroup and shared by its heads through LDS; the elements are requested before the position is looked up, so the
@@ -12,23 +13,12 @@
 // a copy reaches (27 us); one token for 32 requests (40 heads of 64): 3.7 us, three dependent memory round trips.  More
 // units per thread, so that fewer workgroups compute the angles: 2, 3 or 4 of them 41, 37 and 39 us, and 4.3, 4.5 and
 // 4.6 us for the single tokens -- not worth it.
-#include "common.h"
+#include "rotary.h"
 
 namespace feather {
 
 constexpr int kRcThreads = 256;
 constexpr int kRcMaxPairs = 256;      // rot_dim <= 512
-
-// sin and cos of q * pi/2 + r for r in [-pi/4, pi/4]: single-precision minimax polynomials (the decode step's) and the
-// quadrant's signs
-__device__ __forceinline__ void sincos_quadrant(float r, int q, float &s, float &c) {
-    const float r2 = r * r;
-    const float sp = fmaf(r * r2, fmaf(r2, fmaf(r2, -1.9515295891e-4f, 8.3321608736e-3f), -1.6666654611e-1f), r);
-    const float cp = fmaf(r2, fmaf(r2, fmaf(r2, fmaf(r2, 2.443315711809948e-5f, -1.388731625493765e-3f), 4.166664568298827e-2f), -0.5f), 1.0f);
-    const float ss = (q & 1) ? cp : sp, cc = (q & 1) ? sp : cp;
-    s = (q & 2) ? -ss : ss;
-    c = ((q + 1) & 2) ? -cc : cc;
-}
 
 struct RopeChunkArgs {
     const void *qkv;
