@@ -284,7 +284,7 @@ __device__ __forceinline__ void chunk_attn_body(const ChunkArgs &a, int bid) {
 #pragma unroll
         for (int d = 0; d < DB; d++) o[b][d] = float4_t{0.f, 0.f, 0.f, 0.f};
     }
-    const float lazy_raw = kLazy / a.scale_log2e;
+    const float lazy_raw = fminf(kLazy / a.scale_log2e, 3.0e38f);   // finite for any scale: -inf + lazy_raw is -inf
 
     u32x4 kreg[NU];
     uint32_t vreg[NU][4];
@@ -1742,7 +1742,7 @@ extern "C" int feather_paged_chunk_attn_fp8(const void *q, const void *k_cache, 
                   (long long)n_q_heads, (long long)n_kv_heads);
     FEATHER_CHECK(d == 64 || d == 128 || d == 256 || d == 512, FEATHER_ESHAPE, "%s: head dim %lld not supported (64, 128, 256, 512)",
                   me, (long long)d);
-    FEATHER_CHECK(scale > 0.f && scale <= 3.0e38f, FEATHER_EINVAL,
+    FEATHER_CHECK(scale > 0.f && scale <= 2.3e38f, FEATHER_EINVAL,          // scale * log2 e is finite too
                   "%s: scale must be positive and finite (the running maximum is kept on raw scores)", me);
     FEATHER_CHECK(block_size < (1ll << 30) && max_blocks < (1ll << 30) && max_blocks * block_size < (1ll << 30) &&
                       total_rows < (1ll << 30) && n_seq < (1ll << 30) && n_q_heads < (1ll << 20) &&

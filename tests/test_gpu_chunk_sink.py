@@ -38,3 +38,14 @@ def test_many_small_weights_beside_a_large_one(dev, orc, d, lens, ctx, bits):
             worst = ((got - y).abs() / tol).max().item()
             print(d, lens, bits, at, size, "error over bound", worst, "relative", ((got - y).abs() / y.abs()).max().item())
             assert worst <= 1
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-38, 3e-41])
+@pytest.mark.parametrize("d,lens,ctx", [(64, [2], [1500]), (64, [300], [900]), (128, [150], [900]), (256, [3], [1500]), (256, [80], [1500]), (512, [40], [1000])])
+def test_scales_that_leave_all_weights_equal(dev, orc, d, lens, ctx, scale):
+    """Down to subnormal scales the result is the mean of the visible values, in one key range and in several."""
+    P = _problem(orc, 6, lens, ctx, 4, 2, d, 16, "E5M2")
+    y, tol = _reference(P, orc, True, scale=scale)
+    for size in (0, None):
+        got, _ = _run(P, dev, size, 0, scale=scale)
+        assert ((got - y).abs() <= tol).all(), f"workspace of {size} bytes"
