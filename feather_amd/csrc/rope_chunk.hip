@@ -203,6 +203,9 @@ extern "C" int feather_rope_append_chunk(const void *qkv, int src_f16, int64_t r
                       aligned(rot_f32, 16) && aligned(freq_f64, 8) && aligned(cu_seqlens, 4) && aligned(start_pos, 4) &&
                       aligned(block_tables, 4) && aligned(ctx_after, 4) && aligned(seq_status, 4),
                   FEATHER_EINVAL, "%s: misaligned pointer", me);
+    const uintptr_t k0 = reinterpret_cast<uintptr_t>(k_cache), v0 = reinterpret_cast<uintptr_t>(v_cache);
+    FEATHER_CHECK(total_rows == 0 || (uint64_t)(k0 < v0 ? v0 - k0 : k0 - v0) / ((uint64_t)block_size * d) / (uint64_t)n_kv_heads >= (uint64_t)n_blocks,
+                  FEATHER_EINVAL, "%s: k_cache and v_cache overlap", me);
     RopeChunkArgs a;
     a.qkv = qkv; a.cu_seqlens = (const int32_t *)cu_seqlens; a.start_pos = (const int32_t *)start_pos;
     a.block_tables = (const int32_t *)block_tables; a.freq = (const double *)freq_f64; a.q_packed = (uint32_t *)q_packed;

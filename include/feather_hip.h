@@ -364,7 +364,7 @@ int feather_paged_chunk_attn_fp8(const void *q, const void *k_cache, const void 
  *   layout       FEATHER_ROPE_HALF or FEATHER_ROPE_INTERLEAVED
  *   q_packed     [total_rows, n_q, d/4] words; k and v are encoded into the cache at their positions.  A position outside
  *                [0, max_blocks * block_size), or whose table entry is not a block, is not written.  Two rows must not
- *                name the same slot.
+ *                name the same slot; caches that overlap are refused.
  *   ctx_after    [n_seq] tokens in the cache up to the first one that could not be written (start_pos + rows if all were)
  *   seq_status   [n_seq] or NULL: 0 = all written, 1 = some position has no table entry, 2 = some entry is not a block
  *   rot_f32      [total_rows, n_q + 2 n_kv, d] or NULL: the fp32 values the codes were rounded from */
