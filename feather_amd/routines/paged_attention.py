@@ -139,9 +139,10 @@ def paged_chunk_attention_fp8_acc_fp32_gpu(q: torch.Tensor, k_cache: torch.Tenso
     elif (not isinstance(out, torch.Tensor) or out.dtype != out_dtype or tuple(out.shape) != shape
           or out.device != dev or not out.is_contiguous()):
         raise ValueError(f"out must be a contiguous {out_dtype} tensor of shape {shape} on {dev}")
-    elif any(t.data_ptr() < out.data_ptr() + out.nbytes and out.data_ptr() < t.data_ptr() + t.nbytes for t in (q, k_cache, v_cache)):
-        raise ValueError("out overlaps q or a cache, which are read while it is written")
     block_tables, cu_seqlens, ctx_lens = block_tables.contiguous(), cu_seqlens.contiguous(), ctx_lens.contiguous()
+    if not fill and any(t.data_ptr() < out.data_ptr() + out.nbytes and out.data_ptr() < t.data_ptr() + t.nbytes
+                        for t in (q, k_cache, v_cache, block_tables, cu_seqlens, ctx_lens)):
+        raise ValueError("out overlaps q, a cache, the tables or the lengths, which are read while it is written")
     max_blocks = block_tables.shape[1]
     lib = N.lib()
     nbytes = lib.feather_paged_chunk_attn_scratch_bytes(n_seq, total, n_q_heads, n_kv_heads, d, max_blocks * block_size,

@@ -23,3 +23,16 @@ def test_rope_append_into_overlapping_caches():
     assert after.tolist() == [3] and status.tolist() == [0] and both[0].any() and both[1].any()
     q, after, _ = rope_append_chunk(qkv[:0], _z(2), _z(1) + 5, _z(1, 2), pool, pool, n_q_heads=4, freq=freq)   # no rows, nothing written
     assert q.shape == (0, 4, 16) and after.tolist() == [5]
+
+
+def test_attention_result_over_the_tables_or_the_lengths():
+    """The workgroups read them while others already write the result."""
+    from feather_amd.routines.paged_attention import paged_chunk_attention_fp8_acc_fp32_gpu
+    q, kc = _z(3, 4, 16), _z(4, 2, 16, 16)
+    buf = _z(3 * 64 + 8)
+    out = buf[:192].view(3, 64).view(torch.uint32)
+    for bad in (dict(block_tables=buf[190:192].view(1, 2)), dict(cu_seqlens=buf[4:6]), dict(ctx_lens=buf[100:101])):
+        with pytest.raises(ValueError, match="overlaps"):
+            paged_chunk_attention_fp8_acc_fp32_gpu(q, kc, kc, **{**dict(block_tables=_z(1, 2), cu_seqlens=_z(2), ctx_lens=_z(1)), **bad},
+                                                   out_dtype=torch.uint32, out=out)
+    paged_chunk_attention_fp8_acc_fp32_gpu(q, kc, kc, buf[192:194].view(1, 2), buf[194:196], buf[196:197], out_dtype=torch.uint32, out=out)
