@@ -1443,7 +1443,11 @@ __global__ __launch_bounds__(256, wide_shape(D).occ) void chunk_mixed_kernel(Chu
 // lie along DW threads, and zl of these rows of threads take the item's ranges in turn and are joined through LDS, so
 // that few items of many ranges are not one long chain of loads.  Rows of no sequence are zeroed here (fill) or left
 // alone; rows whose kernel had a single range have their result already.
-constexpr int kMergeSeqs = 1024;
+// chunk_plan makes ranges to fill kWideGroups workgroups of the LDS kernel, or up to 3 kCus of the narrow one, with two ranges
+// or more per sequence: a call with ranges has few sequences.  Their offsets are kept in LDS, so the search for a row's sequence
+// is no chain of loads.
+constexpr int kWideGroups = 512, kCus = 256, kMergeSeqs = 512;
+static_assert(kWideGroups / 2 <= kMergeSeqs && 3 * kCus / 2 <= kMergeSeqs, "offsets of more sequences than the merge keeps");
 
 template <int D, int MODE>
 __global__ __launch_bounds__(256) void chunk_merge_kernel(ChunkArgs a, int qt_wide_log2, int bn_wide, int qt_narrow_log2, int zl_log2) {
@@ -1451,11 +1455,8 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(ChunkArgs a, int qt_wi
     __shared__ float4_t x_lds[256];
     __shared__ float2p_t ml_lds[256];
     __shared__ int cu_lds[kMergeSeqs + 1];
-    const bool cached = a.n_seq <= kMergeSeqs;         // the search for the row's sequence then is no chain of loads
-    if (cached)
-        for (int s = threadIdx.x; s <= a.n_seq; s += 256) cu_lds[s] = chunk_clamp_row(a.cu_seqlens[s], a.total_rows);
+    for (int s = threadIdx.x; s <= a.n_seq; s += 256) cu_lds[s] = chunk_clamp_row(a.cu_seqlens[s], a.total_rows);
     __syncthreads();
-    auto cu_at = [&](int s) { return cached ? cu_lds[s] : chunk_clamp_row(a.cu_seqlens[s], a.total_rows); };
     const int tid = threadIdx.x, zl = 1 << zl_log2, w4 = tid % DW, zi = (tid / DW) & (zl - 1);
     const int items = a.total_rows * a.n_q_heads;           // below 2^30
     const int item = (int)blockIdx.x * ((256 / DW) >> zl_log2) + ((tid / DW) >> zl_log2);
@@ -1469,9 +1470,9 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(ChunkArgs a, int qt_wi
         int lo = 0, hi = a.n_seq;                      // last sequence that starts at or before the row
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (cu_at(mid) <= row) lo = mid; else hi = mid;
+            if (cu_lds[mid] <= row) lo = mid; else hi = mid;
         }
-        const int r0 = cu_at(lo), r1 = max(cu_at(lo + 1), r0);
+        const int r0 = cu_lds[lo], r1 = max(cu_lds[lo + 1], r0);
         if (row < r0 || row >= r1) {
             zero = a.fill;
         } else {
@@ -1619,11 +1620,11 @@ static ChunkPlan chunk_plan(int64_t n_seq, int64_t total_rows, int64_t n_q_heads
     const int64_t each = n_seq > 0 ? (total_rows + n_seq - 1) / n_seq * group : 1;   // columns of a sequence of average length
     // 512 workgroups, two per CU: a chunk of 2048 rows, d = 64, 143 + 11 us; 256: 197; 1024: 139 + 14.  16 single rows beside
     // 512 rows, d = 128: 44 + 8 us; 256: 56 + 5; 1024: 54 + 13.
-    p.z_wide = p.wide ? ranges_for(n_seq * ((each + wide_columns(d) - 1) / wide_columns(d)) * n_kv_heads, 512, max_ctx, kChunkMinKeys) : 1;
+    p.z_wide = p.wide ? ranges_for(n_seq * ((each + wide_columns(d) - 1) / wide_columns(d)) * n_kv_heads, kWideGroups, max_ctx, kChunkMinKeys) : 1;
     // the chip holds 256 workgroups of a kernel that fills a CU's registers, two or three times as many of a smaller one
     // (drafts of 32 requests, d = 64, 64 columns: 512 workgroups 24 us, 768 29, 384 28)
     const int weight = (int)(d / 64) * p.nb;
-    const int64_t groups = 256 * (weight <= 2 ? 3 : (weight <= 4 ? 2 : 1));
+    const int64_t groups = kCus * (weight <= 2 ? 3 : (weight <= 4 ? 2 : 1));
     const int64_t tiles = (p.wide ? n_seq : n_seq * ((each + 16 * p.nb - 1) / (16 * p.nb))) * n_kv_heads;
     // twice the even share, for contexts of different lengths
     p.z_narrow = p.narrow && 2 * tiles <= groups ? ranges_for(tiles, 2 * groups, max_ctx, kNarrowMinKeys) : 1;
