@@ -205,8 +205,9 @@ constexpr int kAnyColumns = 1 << 30;   // more columns than a call can have
 // One workgroup (WAVES waves) owns 16 * QB * WAVES columns, each wave 16 * QB of them for the whole key loop.  Tiles
 // of BN keys are fetched packed through the block table into registers two tiles ahead (their block ids three tiles
 // ahead: a table entry is never waited for), decoded into the other LDS buffer one tile ahead, and read by all waves.
-// PAGE4: block_size % 4 == 0, so four keys from a multiple of four on share a block (one table lookup).
-template <int D, int MODE, int QB, int BN, int WAVES, bool PAGE4, bool ZS>
+// PAGE16 (block_size % 16 == 0, the rule of all kernels here): four keys from a multiple of four on share a block, one table
+// lookup.  (Multiples of four would do; block sizes like 12 and 20 take the general path.)
+template <int D, int MODE, int QB, int BN, int WAVES, bool PAGE16, bool ZS>
 __device__ __forceinline__ void chunk_attn_body(const ChunkArgs &a, int bid) {
     constexpr int DW = D / 4;
     constexpr bool BF8 = MODE == FEATHER_E5M2;
@@ -288,14 +289,14 @@ __device__ __forceinline__ void chunk_attn_body(const ChunkArgs &a, int bid) {
 
     u32x4 kreg[NU];
     uint32_t vreg[NU][4];
-    int kid[NU], vid[NU][PAGE4 ? 1 : 4];
+    int kid[NU], vid[NU][PAGE16 ? 1 : 4];
     auto fetch_ids = [&](int key0) {
 #pragma unroll
         for (int i = 0; i < NU; i++) {
             const int u = tid + kThreads * i;
             kid[i] = bt[chunk_block_of(a, min(key0 + u / (D / 16), key_end - 1))];
 #pragma unroll
-            for (int r = 0; r < (PAGE4 ? 1 : 4); r++)
+            for (int r = 0; r < (PAGE16 ? 1 : 4); r++)
                 vid[i][r] = bt[chunk_block_of(a, min(key0 + 4 * (u / DW) + r, key_end - 1))];
         }
     };
@@ -311,7 +312,7 @@ __device__ __forceinline__ void chunk_attn_body(const ChunkArgs &a, int bid) {
             kreg[i] = u32x4{0, 0, 0, 0};
             if (kp < key_end) kreg[i] = *reinterpret_cast<const u32x4 *>(a.k_cache + row_of(kid[i], kp) * DW + 4 * c16);
             const int ddw = u % DW, vp = key0 + 4 * (u / DW);
-            if constexpr (PAGE4) {
+            if constexpr (PAGE16) {
                 const uint32_t *vr = a.v_cache + row_of(vid[i][0], min(vp, key_end - 1) & ~3) * DW + ddw;
 #pragma unroll
                 for (int r = 0; r < 4; r++) vreg[i][r] = vp + r < key_end ? vr[r * DW] : 0u;
