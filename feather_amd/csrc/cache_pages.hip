@@ -18,9 +18,9 @@
 // the compaction plan of 8192 blocks: fewer workgroups, longer serial parts).
 //
 // Copies: 16 bytes a lane, eight caches in flight; bound by the copy rate once there is much to move.  Measured: beams of
-// two requests, 512 blocks, 8 caches 4.4 + 4.3 us (plan, copies; latency only); 256 slots of which 192 go on, 44 caches
-// 9.6 + 14.6 us for 23 MB (six dependent reads before the first copy); compaction of 8192 blocks, 60 % in use, 44 caches
-// 5.2 + 151 us for 709 MB, 4.7 TB/s of the 5.1 that a plain copy of 1 GiB reaches.
+// two requests, 512 blocks, 8 caches 4.6 + 4.9 us (plan, copies; latency only); 256 slots of which 192 go on, 44 caches
+// 9.4 + 14.4 us for 23 MB (six dependent reads before the first copy); compaction of 8192 blocks, 60 % in use, 44 caches
+// 5.0 + 150 us for 709 MB, 4.7 TB/s of the 5.1 that a plain copy of 1 GiB reaches.
 #include "common.h"
 
 namespace feather {

@@ -25,10 +25,10 @@
 // Key ranges share a column out over more workgroups, chunk_merge_kernel adds them up.
 //
 // Measured (a chunk of 2048 rows whose last key is 8192, causal; products and sums of the visible keys, merge included):
-//     d = 64, 32 heads on 4    E5M2 147 + 11 us, 760 TFLOP/s    E4M3 175 + 11 us, 650 TFLOP/s
-//     d = 128, 32 on 8         E5M2 243 us, 990 TFLOP/s         E4M3 317 us, 760 TFLOP/s
-//     d = 256, 8 on 8          E5M2 210 + 14 us, 540 TFLOP/s    E4M3 217 + 14 us, 520 TFLOP/s
-//     d = 512, 8 on 8          E5M2 425 + 26 us, 530 TFLOP/s    E4M3 543 + 26 us, 420 TFLOP/s
+//     d = 64, 32 heads on 4    E5M2 138 + 11 us, 810 TFLOP/s    E4M3 164 + 11 us, 690 TFLOP/s
+//     d = 128, 32 on 8         E5M2 238 us, 1010 TFLOP/s        E4M3 321 us, 750 TFLOP/s
+//     d = 256, 8 on 8          E5M2 202 + 14 us, 560 TFLOP/s    E4M3 211 + 14 us, 530 TFLOP/s
+//     d = 512, 8 on 8          E5M2 415 + 25 us, 550 TFLOP/s    E4M3 539 + 25 us, 430 TFLOP/s
 // (a plain fp16 product of 8192^3 on the same card: 1168).  Bound: vector issue beside the matrix cores up to d = 128 (the
 // exponentials, the decode); LDS reads from d = 256 on (16 columns per wave read every K and V tile once per wave: twice
 // the time of the products), which more columns per wave would halve if the accumulators left registers for them.
@@ -171,7 +171,7 @@ __device__ __forceinline__ void chunk_fill_outside(const ChunkArgs &a, int part,
 constexpr int kChunkFillGroups = 8;    // workgroups of a grid that only look after rows outside every sequence
 // A key range is not cut below this.  LDS kernel: 3 x 97 to 203 rows over 750 to 1501 keys, d = 256: 128 keys 34.5 + 7.6 us
 // (kernel, merge), 256 keys 28.6 + 6.2, 512 keys 37.8 + 4.8.  Narrow kernel: two requests of 211 to 300 keys are done in
-// one range and one launch, 9.9 us; with ranges of 256 keys 8.5 + 4.2.
+// one range and one launch, 6.4 us; with ranges of 256 keys 6.3 + 3.6.
 constexpr int kChunkMinKeys = 256;
 constexpr int kNarrowMinKeys = 512;
 constexpr int kNarrowStep = 128;       // keys that the four waves of a narrow workgroup take per turn
@@ -916,10 +916,12 @@ __device__ __forceinline__ void chunk_attn32_body(const ChunkArgs &a, int bid) {
 // only.
 // RING = 0 (any block size): rows go to registers, NF steps in flight, an address for every key.
 // Each wave keeps its own reference point and sums; they are joined through LDS, and the ranges by the merge kernel.
-// Measured: 16 rows of 32 heads on 8 at context 65537, d = 128, E4M3 47 + 6 us for 134 MB, 2.9 TB/s in the kernel (E5M2
-// 39 + 6 us); 32 requests with 3 to 8 rows, contexts to 4096, 32 heads on 4, d = 64, E4M3 24 + 5 us for 39 MB: a wave has
-// five steps there, and the round trips in front of them (lengths, block ids, rows), the exponentials of 64 columns and the
-// join bound it.  Registers instead of the ring (RING = 0 everywhere): 51 and 34 us.
+// Measured: 16 rows of 32 heads on 8 at context 65537, d = 128, E4M3 48 + 5 us (E5M2 38 + 5): two tiles of 32 columns, each of
+// which requests and decodes the 134 MB of the cache for itself, 2.8 TB/s of different bytes (one tile of 64 columns 45 us, but
+// see narrow_blocks); 32 requests with 3 to 8 rows, contexts to 4096, 32 heads on 4, d = 64, E4M3 24 + 5 us for 39 MB: a wave
+// has five steps there, and the round trips in front of them (lengths, block ids, rows), the exponentials of 64 columns and
+// the join bound it.  Blocks that are no multiples of 16, through registers: blocks of 20 at context 65537 57 + 5 us, the 32
+// requests with blocks of 8 or 20 25 + 4 us.
 template <int D>
 struct NarrowStep {
     u32x4 kw[2][D / 64];
@@ -1619,8 +1621,9 @@ static ChunkPlan chunk_plan(int64_t n_seq, int64_t total_rows, int64_t n_q_heads
     }
     p.narrow_rows = p.wide && p.narrow ? (int)(p.col_split / group) : 0;
     const int64_t each = n_seq > 0 ? (total_rows + n_seq - 1) / n_seq * group : 1;   // columns of a sequence of average length
-    // 512 workgroups, two per CU: a chunk of 2048 rows, d = 64, 143 + 11 us; 256: 197; 1024: 139 + 14.  16 single rows beside
-    // 512 rows, d = 128: 44 + 8 us; 256: 56 + 5; 1024: 54 + 13.
+    // 512 workgroups, two per CU: a chunk of 2048 rows, d = 64, 142 + 11 us; 256: 198; 1024: 141 + 14.  16 single rows beside
+    // 512 rows, d = 128, 136 tiles: 512 are three ranges, 43.6 + 8.2 us; 256 one, 56 + 5; 272 two, 42.1 + 7.6; 1024 seven,
+    // 54 + 13.  (The workgroups of the narrow part in the same grid are not counted.)
     p.z_wide = p.wide ? ranges_for(n_seq * ((each + wide_columns(d) - 1) / wide_columns(d)) * n_kv_heads, kWideGroups, max_ctx, kChunkMinKeys) : 1;
     // the chip holds 256 workgroups of a kernel that fills a CU's registers, two or three times as many of a smaller one
     // (drafts of 32 requests, d = 64, 64 columns: 512 workgroups 24 us, 768 29, 384 28)

@@ -10,9 +10,9 @@
 // A streaming kernel, bound by its bytes: 4 (or 2) in, 1 out per element.  The angles of a token are computed once per
 // workgroup and shared by its heads through LDS; the elements are requested before the position is looked up, so the
 // two chains overlap.  9 ragged chunks (4505 rows of 48 heads, d = 128, fp32): 138 MB in 37 us, 3.7 TB/s of the 5.1 that
-// a copy reaches (27 us); one token for 32 requests (40 heads of 64): 3.7 us, three dependent memory round trips.  More
-// units per thread, so that fewer workgroups compute the angles: 2, 3 or 4 of them 41, 37 and 39 us, and 4.3, 4.5 and
-// 4.6 us for the single tokens -- not worth it.
+// a copy reaches (27 us), from fp16 83 MB in 32 us; one token for 32 requests (40 heads of 64): 3.7 us, three dependent
+// memory round trips.  More units per thread, so that fewer workgroups compute the angles: 2, 3 or 4 of them 41, 37 and
+// 39 us, and 4.3, 4.5 and 4.6 us for the single tokens -- not worth it.
 #include "rotary.h"
 
 namespace feather {
