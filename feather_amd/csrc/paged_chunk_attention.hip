@@ -32,6 +32,7 @@
 // (a plain fp16 product of 8192^3 on the same card: 1168).  Bound: vector issue beside the matrix cores up to d = 128 (the
 // exponentials, the decode); LDS reads from d = 256 on (16 columns per wave read every K and V tile once per wave: twice
 // the time of the products), which more columns per wave would halve if the accumulators left registers for them.
+#include <cmath>
 #include <type_traits>
 
 #include "common.h"
@@ -57,6 +58,7 @@ struct ChunkArgs {
     float *part_narrow;               // its partial results, then the (maximum, sum) pairs, then the keys per range
     int col_split;                    // sequences of more columns than this take the LDS kernel, the others the narrow one
     float scale_log2e;
+    float shift_raw, raise_raw;       // kShift and kShift + kLazy as differences of raw scores
 };
 
 // What a tile of `qt` columns works on: its sequence, and how many keys its columns can see.
@@ -199,6 +201,15 @@ __device__ __forceinline__ int narrow_min_keys(const ChunkArgs &a, int qt) {
 constexpr float kShift = 8.f, kGuard = 61440.f;
 constexpr float kLazy = 7.f;           // the kernel that compares maxima raises the reference beyond 2^kLazy: P to 2^(kShift + kLazy) = 32768
 __device__ __forceinline__ float chunk_reference(float m, float scale_log2e) { return __builtin_fmaf(m, scale_log2e, -kShift); }
+// The exponent is one fused operation, s c - (m c - kShift), whose second operand is rounded: by 2^-10 at kFar, by more than 16
+// for the largest E5M2 codes, where P of the maximum itself would overflow or vanish.  Columns whose reference is beyond kFar
+// subtract the maximum first, (s - m) c + kShift, one operation more: they take the path of a raised reference with every
+// tile.  The 16x16 LDS kernel (d = 256, 512), which LDS reads bound, always subtracts first (0 to 1 % of its time).
+constexpr float kFar = 16384.f;
+template <bool FAR>
+__device__ __forceinline__ float chunk_exp(float s, float scale_log2e, float ref) {   // ref: the maximum (FAR), or as chunk_reference gives it
+    return __builtin_amdgcn_exp2f(FAR ? __builtin_fmaf(s - ref, scale_log2e, kShift) : __builtin_fmaf(s, scale_log2e, -ref));
+}
 constexpr int kAnyColumns = 1 << 30;   // more columns than a call can have
 
 // ---- tiles through LDS --------------------------------------------------------------------------------------------
@@ -285,7 +296,6 @@ __device__ __forceinline__ void chunk_attn_body(const ChunkArgs &a, int bid) {
 #pragma unroll
         for (int d = 0; d < DB; d++) o[b][d] = float4_t{0.f, 0.f, 0.f, 0.f};
     }
-    const float lazy_raw = fminf(kLazy / a.scale_log2e, 3.0e38f);   // finite for any scale: -inf + lazy_raw is -inf
 
     u32x4 kreg[NU];
     uint32_t vreg[NU][4];
@@ -444,12 +454,13 @@ __device__ __forceinline__ void chunk_attn_body(const ChunkArgs &a, int bid) {
                     mx = max3_raw(mx, s[b][c][2], s[b][c][3]);
                 }
                 mx = max_xor32(max_xor16(mx));
-                // The reference point is raised only when a column exceeds it by 2^kLazy (O / l does not depend on it).  A
+                // m_run is the point that P refers to, kShift below the maximum (at it where the scores are so large that the
+                // difference would be rounded up).  It is raised only when a column exceeds it by 2^(kShift + kLazy).  A
                 // column that has seen no key yet keeps -inf and refers to zero: its scores are -inf, its P zero.
                 const float m_old = m_run[b];
-                const bool raise = __builtin_amdgcn_ballot_w64(mx > m_old + lazy_raw) != 0;
-                const float m_new = raise ? max_raw(m_old, mx) : m_old;
-                const float mc = m_new == -INFINITY ? 0.f : chunk_reference(m_new, a.scale_log2e);
+                const bool raise = __builtin_amdgcn_ballot_w64(mx - m_old > a.raise_raw) != 0;
+                const float low = mx - a.shift_raw, m_new = raise ? max_raw(m_old, mx - low > 1.1f * a.shift_raw ? mx : low) : m_old;
+                const float ref = m_new == -INFINITY ? 0.f : m_new;
                 if (raise) {
                     const float alpha = m_old == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_old - m_new) * a.scale_log2e);
                     m_run[b] = m_new;
@@ -463,8 +474,8 @@ __device__ __forceinline__ void chunk_attn_body(const ChunkArgs &a, int bid) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const float4_t &x = s[b][2 * g + (i >> 1)];
-                        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * (i & 1)], a.scale_log2e, -mc));
-                        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * (i & 1) + 1], a.scale_log2e, -mc));
+                        const float e0 = __builtin_amdgcn_exp2f((x[2 * (i & 1)] - ref) * a.scale_log2e);   // (subtracted first: see kFar)
+                        const float e1 = __builtin_amdgcn_exp2f((x[2 * (i & 1) + 1] - ref) * a.scale_log2e);
                         pw[i] = as_u32(__builtin_convertvector(float2p_t{e0, e1}, half2_t));
                         l_run[b] = dot2(pw[i], 0x3c003c00u, l_run[b]);   // the sum takes the rounded values that multiply V
                     }
@@ -799,15 +810,16 @@ __device__ __forceinline__ void chunk_attn32_body(const ChunkArgs &a, int bid) {
                 }
                 // P against the column's current reference point; the lane's share of the sum tells whether that was safe
                 // (see kGuard); if not, the reference is raised to the true maximum and P computed again
-                auto exp_block = [&](const float mc) {
+                auto exp_block = [&](auto far_c, const float ref) {
+                    constexpr bool FAR = decltype(far_c)::value;
                     float sum = 0.f;
 #pragma unroll
                     for (int g = 0; g < 4; g++) {
                         uint32_t pw[4];
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
-                            const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][g >> 1][8 * (g & 1) + 2 * i], a.scale_log2e, -mc));
-                            const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][g >> 1][8 * (g & 1) + 2 * i + 1], a.scale_log2e, -mc));
+                            const float e0 = chunk_exp<FAR>(sc[b][g >> 1][8 * (g & 1) + 2 * i], a.scale_log2e, ref);
+                            const float e1 = chunk_exp<FAR>(sc[b][g >> 1][8 * (g & 1) + 2 * i + 1], a.scale_log2e, ref);
                             pw[i] = as_u32(__builtin_convertvector(float2p_t{e0, e1}, half2_t));
                             sum = dot2(pw[i], 0x3c003c00u, sum);  // the sum takes the rounded values that multiply V
                         }
@@ -815,7 +827,7 @@ __device__ __forceinline__ void chunk_attn32_body(const ChunkArgs &a, int bid) {
                     }
                     return sum;
                 };
-                float sum = exp_block(mc_run[b]);
+                float sum = exp_block(std::false_type{}, mc_run[b]);
                 if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(sum < kGuard)) != 0, 0)) {
                     float mx = max3_raw(sc[b][0][0], sc[b][0][1], sc[b][0][2]);
                     mx = max_raw(mx, sc[b][0][3]);
@@ -825,12 +837,15 @@ __device__ __forceinline__ void chunk_attn32_body(const ChunkArgs &a, int bid) {
                     const float m_old = m_run[b], m_new = max_raw(m_old, mx);
                     // a column that has seen no key keeps the reference -inf: its scores are -inf here, its P zero
                     const float alpha = m_old == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_old - m_new) * a.scale_log2e);
+                    const float mc = chunk_reference(m_new, a.scale_log2e);
+                    const bool far = m_new != -INFINITY && __builtin_fabsf(mc) > kFar;
                     m_run[b] = m_new;
-                    mc_run[b] = chunk_reference(m_new, a.scale_log2e);
+                    mc_run[b] = far ? -INFINITY : mc;             // (-inf: such a column comes here with every tile)
                     l_run[b] *= alpha;
 #pragma unroll
                     for (int d = 0; d < DB; d++) o[b][d] *= alpha;
-                    sum = exp_block(m_new == -INFINITY ? 0.f : mc_run[b]);
+                    if (__builtin_amdgcn_ballot_w64(far) != 0) sum = exp_block(std::true_type{}, m_new == -INFINITY ? 0.f : m_new);
+                    else sum = exp_block(std::false_type{}, m_new == -INFINITY ? 0.f : mc);
                 }
                 l_run[b] += sum;
                 if constexpr (D == 64)
@@ -1195,13 +1210,14 @@ __device__ __forceinline__ void chunk_narrow_body(const ChunkArgs &a, int pair, 
         // was safe (see kGuard).  If not -- the first keys of a column, whose reference is -inf, or a score far above it --
         // the references are raised to the true maxima, the accumulators rescaled and P computed again.
         float sum[NB];
-        auto exp_block = [&](int b, float mc) {
+        auto exp_block = [&](auto far_c, int b, float ref) {
+            constexpr bool FAR = decltype(far_c)::value;
             uint32_t pw[4];
             sum[b] = 0.f;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][i >> 1][2 * (i & 1)], a.scale_log2e, -mc));
-                const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][i >> 1][2 * (i & 1) + 1], a.scale_log2e, -mc));
+                const float e0 = chunk_exp<FAR>(sc[b][i >> 1][2 * (i & 1)], a.scale_log2e, ref);
+                const float e1 = chunk_exp<FAR>(sc[b][i >> 1][2 * (i & 1) + 1], a.scale_log2e, ref);
                 pw[i] = as_u32(__builtin_convertvector(float2p_t{e0, e1}, half2_t));
                 sum[b] = dot2(pw[i], 0x3c003c00u, sum[b]);              // the sum takes the rounded values that multiply V
             }
@@ -1210,7 +1226,7 @@ __device__ __forceinline__ void chunk_narrow_body(const ChunkArgs &a, int pair, 
         bool safe = true;
 #pragma unroll
         for (int b = 0; b < NB; b++) {
-            exp_block(b, mc_run[b]);
+            exp_block(std::false_type{}, b, mc_run[b]);
             safe = safe && sum[b] < kGuard;
         }
         if (__builtin_expect(__builtin_amdgcn_ballot_w64(!safe) != 0, 0)) {
@@ -1223,14 +1239,17 @@ __device__ __forceinline__ void chunk_narrow_body(const ChunkArgs &a, int pair, 
                 const float m_old = m_run[b], m_new = max_raw(m_old, mx);
                 // a column that has seen no key keeps the reference -inf: its scores are -inf here, its P zero
                 const float alpha = m_old == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_old - m_new) * a.scale_log2e);
+                const float mc = chunk_reference(m_new, a.scale_log2e);
+                const bool far = m_new != -INFINITY && __builtin_fabsf(mc) > kFar;
                 m_run[b] = m_new;
-                mc_run[b] = chunk_reference(m_new, a.scale_log2e);
+                mc_run[b] = far ? -INFINITY : mc;                       // (-inf: such a column comes here with every step)
                 l_run[b] *= alpha;
 #pragma unroll
                 for (int rb = 0; rb < RB; rb++)
 #pragma unroll
                     for (int c = 0; c < 4; c++) o[b][rb][c] *= alpha;
-                exp_block(b, m_new == -INFINITY ? 0.f : mc_run[b]);
+                if (__builtin_amdgcn_ballot_w64(far) != 0) exp_block(std::true_type{}, b, m_new == -INFINITY ? 0.f : m_new);
+                else exp_block(std::false_type{}, b, m_new == -INFINITY ? 0.f : mc);
             }
         }
 #pragma unroll
@@ -1787,6 +1806,8 @@ extern "C" int feather_paged_chunk_attn_fp8(const void *q, const void *k_cache, 
     a.z_wide = p.z_wide; a.z_narrow = p.z_narrow; a.per_group = p.per_group; a.narrow_rows = p.narrow_rows; a.narrow_tiles = p.tiles;
     a.part_narrow = reinterpret_cast<float *>(static_cast<char *>(scratch) + chunk_wide_scratch(p)); a.col_split = p.col_split;
     a.scale_log2e = scale * 1.4426950408889634f;
+    a.shift_raw = std::fmin(kShift / a.scale_log2e, 1.0e38f);          // (finite for a subnormal scale too)
+    a.raise_raw = std::fmin((kShift + kLazy) / a.scale_log2e, 3.0e38f);
     hipStream_t s = (hipStream_t)stream;
     const bool al = block_size % 16 == 0;
     if (mode == FEATHER_E5M2) return al ? dispatch_chunk<FEATHER_E5M2, true>(a, p, d, s) : dispatch_chunk<FEATHER_E5M2, false>(a, p, d, s);
