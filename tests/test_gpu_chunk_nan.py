@@ -66,3 +66,25 @@ def test_nan_in_a_key(dev, orc, shape):
         P = _problem(orc, 32, *shape[:6], "E5M2")
         P["kc"].view(np.uint8).reshape(-1, Hkv, bs, d)[P["bt"][0, at // bs], 0, at % bs, 7] = NAN
         _agree(P, dev, orc, shape[6])
+
+
+@pytest.mark.parametrize("code", [0x7C, 0xFC])
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: f"d{s[4]}_bs{s[5]}_rows{sum(s[0])}_ctx{max(s[1])}")
+def test_infinite_key(dev, orc, shape, code):
+    """A score of +inf makes the row NaN (inf - inf), one of -inf a weight of zero, also where a range has no other."""
+    lens, ctx, Hq, Hkv, d, bs = shape[:6]
+    n, c = lens[0], ctx[0]
+    for at in sorted({x for x in (256, 1536, c - n + n // 2) if c - n <= x < c}):
+        P = _problem(orc, 33, *shape[:6], "E5M2")
+        P["kc"].view(np.uint8).reshape(-1, Hkv, bs, d)[P["bt"][0, at // bs], 0, at % bs, 7] = code
+        P["q"].view(np.uint8).reshape(P["total"], Hq, d)[0, 0, 7] = 0x3C          # both signs of scores, whatever the draw
+        P["q"].view(np.uint8).reshape(P["total"], Hq, d)[lens[0] - 1, 0, 7] = 0x3C if code == 0x7C else 0xBC
+        P["q"].view(np.uint8).reshape(P["total"], Hq, d)[lens[0] - 1, (Hq // Hkv) - 1, 7] = 0xBC if code == 0x7C else 0x3C
+        if Hq // Hkv > 1:
+            _agree(P, dev, orc, shape[6])
+        else:                                              # one head per KV head: the last row has a score of -inf
+            y, tol = _reference(P, orc, True)
+            nan = torch.isnan(y)
+            for size in (None, 0):
+                got, _ = _run(P, dev, size, 0)
+                assert torch.equal(torch.isnan(got), nan) and ((got - y).abs()[~nan] <= tol[~nan]).all()
