@@ -25,10 +25,10 @@
 // Key ranges share a column out over more workgroups, chunk_merge_kernel adds them up.
 //
 // Measured (a chunk of 2048 rows whose last key is 8192, causal; products and sums of the visible keys, merge included):
-//     d = 64, 32 heads on 4    E5M2 138 + 11 us, 810 TFLOP/s    E4M3 164 + 11 us, 690 TFLOP/s
+//     d = 64, 32 heads on 4    E5M2 137 + 11 us, 810 TFLOP/s    E4M3 164 + 11 us, 690 TFLOP/s
 //     d = 128, 32 on 8         E5M2 238 us, 1010 TFLOP/s        E4M3 321 us, 750 TFLOP/s
-//     d = 256, 8 on 8          E5M2 202 + 14 us, 560 TFLOP/s    E4M3 211 + 14 us, 530 TFLOP/s
-//     d = 512, 8 on 8          E5M2 415 + 25 us, 550 TFLOP/s    E4M3 539 + 25 us, 430 TFLOP/s
+//     d = 256, 8 on 8          E5M2 197 + 14 us, 570 TFLOP/s    E4M3 211 + 14 us, 530 TFLOP/s
+//     d = 512, 8 on 8          E5M2 414 + 26 us, 550 TFLOP/s    E4M3 545 + 25 us, 420 TFLOP/s
 // (a plain fp16 product of 8192^3 on the same card: 1168).  Bound: vector issue beside the matrix cores up to d = 128 (the
 // exponentials, the decode); LDS reads from d = 256 on (16 columns per wave read every K and V tile once per wave: twice
 // the time of the products), which more columns per wave would halve if the accumulators left registers for them.
